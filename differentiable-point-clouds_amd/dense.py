@@ -1,0 +1,392 @@
+"""The dense layers around the projector: their product in 8 bits, and the orthogonalised update of their weights.
+
+    y = linear_fp8(x, weight, bias)              # differentiable; weight a tensor, or packed once with pack_weight_fp8
+    layer = Fp8Linear(1024, 24000)               # torch.nn.Linear whose products run in 8 bits
+    o = newton_schulz(g)                         # a matrix, a batch of them or a list: (nearly) orthogonal factors
+    muon_update(weights, grads, momenta, lr=...) # one optimiser step in place (optim.Muon calls it)
+
+The reference leaves both to stock TensorFlow: fully connected layers (dpc/nets/img_encoder.py:11-50, pc_decoder.py:5-42) and
+its optimiser (dpc/run/train.py:86-92).  Kernels: csrc/dense, C ABI: include/dpc_dense.h.  Calls only enqueue work on the current
+stream of the tensors' device, allocate through torch, and can be recorded into a HIP graph."""
+import collections
+import contextlib
+import ctypes
+import math
+
+import torch
+
+from . import _dense_capi, ops
+from ._dense_capi import BLOCK, DpcDenseMatrix, DpcDenseSteps
+
+_CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+
+
+# ---------------------------------------------------------------------------
+# helpers
+# ---------------------------------------------------------------------------
+def _library(*tensors):
+    """the active library, after checking that every tensor (None aside) lies where it computes, on one device"""
+    lib, device = _dense_capi.get_library(), None
+    for t in tensors:
+        if t is None:
+            continue
+        if not isinstance(t, torch.Tensor):
+            raise TypeError("expected a torch.Tensor, got %r" % type(t))
+        if t.layout != torch.strided:
+            raise TypeError("expected a dense tensor, got layout %s" % t.layout)
+        if lib.host_memory:
+            if t.is_cuda:
+                raise ValueError("emulation library needs host tensors")
+        elif not t.is_cuda:
+            raise ValueError("the dense operators need tensors on a ROCm device (no CPU fallback)")
+        if device is not None and t.device != device:
+            raise ValueError("tensors on different devices: %s and %s" % (device, t.device))
+        device = t.device
+    return lib
+
+
+def _code(t, what):
+    if t.dtype not in _CODES:
+        raise TypeError("%s must be float32, bfloat16 or float16, got %s" % (what, t.dtype))
+    return _CODES[t.dtype]
+
+
+def _on(lib, device):
+    """(context that makes `device` current, its current stream)"""
+    if lib.host_memory:
+        return contextlib.nullcontext(), None
+    return torch.cuda.device(device), torch.cuda.current_stream(device).cuda_stream
+
+
+def _bytes(n, device):
+    """n bytes, 256-byte aligned: (tensor that owns them, address)"""
+    t = torch.empty(n + 256, dtype=torch.uint8, device=device)
+    if ops._POISON:
+        t.fill_(255)
+    return t, (t.data_ptr() + 255) & ~255
+
+
+def _buffer(shape, dtype, device):
+    t = torch.empty(shape, dtype=dtype, device=device)
+    if ops._POISON:
+        t.view(torch.uint8).fill_(255)
+    return t
+
+
+def _rows(t):
+    """t [rows, cols] with neighbouring columns and rows that do not overlap"""
+    if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+        return t.contiguous()
+    return t
+
+
+# ---------------------------------------------------------------------------
+# the product
+# ---------------------------------------------------------------------------
+class Fp8Weight(collections.namedtuple("Fp8Weight", ["values", "scales", "in_features"])):
+    """A weight [out_features, in_features] in 8 bits, laid out once for serving.
+
+    values  float8_e4m3fn [out_features, 128 * blocks], blocks = ceil(in_features / 128); zeros behind in_features
+    scales  uint8 [blocks, out_features]: the 128 values of a block stand for value * 2^(scale - 127)"""
+    __slots__ = ()
+
+    @property
+    def out_features(self):
+        return self.values.shape[0]
+
+
+def _check_packed(w):
+    blocks = -(-int(w.in_features) // BLOCK)
+    if w.in_features < 0 or w.values.dim() != 2 or w.values.dtype != torch.float8_e4m3fn or w.values.shape[1] != blocks * BLOCK:
+        raise ValueError("values must be float8_e4m3fn [out_features, %d], got %s %s" % (blocks * BLOCK, w.values.dtype, tuple(w.values.shape)))
+    if w.scales.dtype != torch.uint8 or tuple(w.scales.shape) != (blocks, w.values.shape[0]):
+        raise ValueError("scales must be uint8 [%d, %d], got %s %s" % (blocks, w.values.shape[0], w.scales.dtype, tuple(w.scales.shape)))
+    if not (w.values.is_contiguous() and w.scales.is_contiguous()) or w.values.data_ptr() % 16:
+        raise ValueError("values and scales must be contiguous, values 16-byte aligned")
+
+
+def _quantize(lib, t, along_cols, along_rows, sums=False):
+    """t [rows, cols] in 8 bits: ((values, scales) with blocks along the columns | None, the same of the transposed matrix | None,
+    sums of each 128 rows | None)"""
+    rows, cols = t.shape
+    dev = t.device
+    nc, nr = -(-cols // BLOCK), -(-rows // BLOCK)
+    q = s = qt = st = cs = None
+    if along_cols:
+        q, s = _buffer((rows, nc * BLOCK), torch.float8_e4m3fn, dev), _buffer((nc, rows), torch.uint8, dev)
+    if along_rows:
+        qt, st = _buffer((cols, nr * BLOCK), torch.float8_e4m3fn, dev), _buffer((nr, cols), torch.uint8, dev)
+        if sums:
+            cs = _buffer((nr, cols), torch.float32, dev)
+    guard, stream = _on(lib, dev)
+    p = ops._ptr
+    with guard:
+        lib.check(lib.dpc_dense_quantize(stream, rows, cols, _CODES[t.dtype], t.data_ptr(), t.stride(0) if rows > 1 else cols, p(q), p(s),
+                                         p(qt), p(st), p(cs)), "dpc_dense_quantize")
+    return (q, s), (qt, st), cs
+
+
+def _product(lib, a, b, bias, dtype):
+    """[rows of a, rows of b] = a b^T (+ bias) of two 8-bit forms with blocks along the summed axis"""
+    (qa, sa), (qb, sb) = a, b
+    m, n, blocks = qa.shape[0], qb.shape[0], sa.shape[0]
+    out = _buffer((m, n), dtype, qa.device)
+    code = _CODES[dtype]
+    need = lib.dpc_dense_product_workspace(m, n, blocks, code)
+    hold, ws = _bytes(need, qa.device) if need else (None, None)
+    guard, stream = _on(lib, qa.device)
+    with guard:
+        lib.check(lib.dpc_dense_product(stream, m, n, blocks, qa.data_ptr(), sa.data_ptr(), qb.data_ptr(), sb.data_ptr(), ops._ptr(bias),
+                                        0 if bias is None else _CODES[bias.dtype], out.data_ptr(), code, ws, need), "dpc_dense_product")
+    return out
+
+
+class _LinearFp8(torch.autograd.Function):
+    """y = Q(x) Q(w)^T + bias.  The gradients are those of the product of the held values, with dy held in 8 bits too, each in
+    blocks along the axis that its product sums over: dx = Q(dy) Q(w^T)^T, dw = Q(dy^T) Q(x^T)^T, dbias = sum of dy's rows."""
+
+    @staticmethod
+    def forward(ctx, x, w, bias):
+        lib = _library(x, w, bias)
+        need_x, need_w, need_b = ctx.needs_input_grad
+        xq, xt, _ = _quantize(lib, _rows(x), True, need_w)
+        wq, wt, _ = _quantize(lib, _rows(w), True, need_x)
+        ctx.meta = (w.dtype, None if bias is None else bias.dtype)
+        ctx.save_for_backward(*xt, *wt)
+        return _product(lib, xq, wq, bias, x.dtype)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        need_x, need_w, need_b = ctx.needs_input_grad
+        w_dtype, b_dtype = ctx.meta
+        xq, xs, wq, ws = ctx.saved_tensors
+        lib = _library(dy)
+        dq, dt, sums = _quantize(lib, _rows(dy), need_x, need_w or need_b, need_b)
+        dx = _product(lib, dq, (wq, ws), None, dy.dtype) if need_x else None
+        dw = _product(lib, dt, (xq, xs), None, w_dtype) if need_w else None
+        db = None
+        if need_b:
+            db = _buffer((dy.shape[1],), b_dtype, dy.device)
+            guard, stream = _on(lib, dy.device)
+            with guard:
+                lib.check(lib.dpc_dense_colsum(stream, sums.shape[0], dy.shape[1], sums.data_ptr(), _CODES[b_dtype], db.data_ptr()),
+                          "dpc_dense_colsum")
+        return dx, dw, db
+
+
+def pack_weight_fp8(weight):
+    """The 8-bit form of ``weight`` [out_features, in_features], to be kept for calls of ``linear_fp8``."""
+    lib = _library(weight)
+    _code(weight, "weight")
+    if weight.dim() != 2:
+        raise ValueError("weight must be [out_features, in_features], got %s" % (tuple(weight.shape),))
+    (q, s), _, _ = _quantize(lib, _rows(weight.detach()), True, False)
+    return Fp8Weight(q, s, weight.shape[1])
+
+
+def linear_fp8(x, weight, bias=None):
+    """x [..., in_features] times weight^T, both held in 8 bits (e4m3) with one power-of-two scale for each 128 neighbours along
+    the summed axis; the result has x's type.  Sums are held in 32 bits; results of 16 bits take the 8-bit matrix instruction
+    (whose sums are off by 1.4e-5 of the result), float32 results the half-precision one (1e-7).
+
+    ``weight`` [out_features, in_features], float32, bfloat16 or float16 (not necessarily x's type): differentiable in x, weight
+    and bias, once; the gradients' products run in 8 bits as well.  ``weight`` an ``Fp8Weight``: serving; x must not require a
+    gradient.  A value that is not finite makes NaN of every result that it enters.  float32 magnitudes are meant to lie within
+    2^-100 .. 2^100."""
+    packed = isinstance(weight, Fp8Weight)
+    lib = _library(x, weight.values if packed else weight, weight.scales if packed else None, bias)
+    _code(x, "x")
+    if packed:
+        _check_packed(weight)
+        n, k = weight.out_features, int(weight.in_features)
+    else:
+        _code(weight, "weight")
+        if weight.dim() != 2:
+            raise ValueError("weight must be [out_features, in_features], got %s" % (tuple(weight.shape),))
+        n, k = weight.shape
+    if x.dim() < 1 or x.shape[-1] != k:
+        raise ValueError("x must be [..., %d], got %s" % (k, tuple(x.shape)))
+    if bias is not None:
+        _code(bias, "bias")
+        if tuple(bias.shape) != (n,):
+            raise ValueError("bias must be [%d], got %s" % (n, tuple(bias.shape)))
+        bias = bias.contiguous()
+    lead = x.shape[:-1]
+    rows = math.prod(lead)
+    x2 = x.reshape(rows, k)
+    if not packed:
+        return _LinearFp8.apply(x2, weight, bias).reshape(*lead, n)
+    if torch.is_grad_enabled() and (x.requires_grad or bias is not None and bias.requires_grad):
+        raise ValueError("a packed weight serves only: call under torch.no_grad(), or pass the weight itself")
+    xq, _, _ = _quantize(lib, _rows(x2), True, False)
+    return _product(lib, xq, (weight.values, weight.scales), bias, x.dtype).reshape(*lead, n)
+
+
+class Fp8Linear(torch.nn.Linear):
+    """torch.nn.Linear whose product and gradients run in 8 bits (``linear_fp8``); weights and optimiser state keep their type."""
+
+    def forward(self, x):
+        return linear_fp8(x, self.weight, self.bias)
+
+
+# ---------------------------------------------------------------------------
+# orthogonalisation and the update
+# ---------------------------------------------------------------------------
+def _steps_of(steps, coefficients, eps):
+    if isinstance(steps, bool) or not isinstance(steps, int) or not 1 <= steps <= _dense_capi.MAX_STEPS:
+        raise ValueError("steps must be a whole number in 1 .. %d, got %r" % (_dense_capi.MAX_STEPS, steps))
+    if not (eps > 0 and math.isfinite(eps)):
+        raise ValueError("eps must be positive, got %r" % (eps,))
+    coefficients = tuple(coefficients)
+    if len(coefficients) == 3 and not any(hasattr(c, "__len__") for c in coefficients):
+        coefficients = (coefficients,) * steps
+    if len(coefficients) != steps or any(len(c) != 3 for c in coefficients):
+        raise ValueError("coefficients must be (a, b, c), or one such triple for each of the %d steps" % steps)
+    s = DpcDenseSteps()
+    s.steps, s.eps = steps, float(eps)
+    for i, abc in enumerate(coefficients):
+        s.coefficients[i][0], s.coefficients[i][1], s.coefficients[i][2] = (float(v) for v in abc)
+    return s
+
+
+def _run_orthogonal(lib, device, dtype, entries, steps):
+    """entries: (grad, momentum | None, out, rows, cols, scale) with contiguous storage"""
+    guard, stream = _on(lib, device)
+    code = _CODES[dtype]
+    for at in range(0, len(entries), _dense_capi.MAX_MATRICES):
+        part = entries[at:at + _dense_capi.MAX_MATRICES]
+        ms = (DpcDenseMatrix * len(part))()
+        for m, (g, mom, out, rows, cols, scale) in zip(ms, part):
+            m.grad, m.momentum, m.out, m.rows, m.cols, m.scale = g.data_ptr(), ops._ptr(mom), out.data_ptr(), rows, cols, scale
+        need = lib.dpc_dense_orthogonal_workspace(len(part), ms, code)
+        hold, ws = _bytes(need, device)
+        with guard:
+            lib.check(lib.dpc_dense_orthogonal(stream, len(part), ms, code, ctypes.byref(steps), ws, need), "dpc_dense_orthogonal")
+
+
+def newton_schulz(grads, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
+    """X0 = G / (|G| + eps) (Frobenius norm), then ``steps`` times X <- (a I + b A + c A^2) X with A = X X^T (X turned so that it
+    is at least as wide as tall): with the default coefficients the singular values move to about 1.
+
+    ``grads``: a tensor [..., rows, cols], or a list of matrices of any sizes; all of a list run in the same launches.  The result
+    has the same form and type; no gradient flows.  float32 and float16 compute to single precision's accuracy, bfloat16
+    to its own.  ``coefficients``: (a, b, c), or a triple for each step; refused where the scalar iteration leaves (-3.5, 3.5)."""
+    single = isinstance(grads, torch.Tensor)
+    mats = [grads] if single else list(grads)
+    lib = _library(*mats)
+    s = _steps_of(steps, coefficients, eps)
+    for g in mats:
+        _code(g, "a matrix")
+        if g.dim() < 2 or not single and g.dim() != 2:
+            raise ValueError("expected %s, got %s" % ("[..., rows, cols]" if single else "matrices", tuple(g.shape)))
+    with torch.no_grad():
+        sources = [g.detach().contiguous() for g in mats]
+        outs = [_buffer(g.shape, g.dtype, g.device) for g in sources]
+        by_type = {}
+        for g, o in zip(sources, outs):
+            if not g.numel():
+                continue
+            rows, cols = g.shape[-2:]
+            for a, b in zip(g.reshape(-1, rows, cols).unbind(0), o.view(-1, rows, cols).unbind(0)):
+                by_type.setdefault(g.dtype, []).append((a, None, b, rows, cols, 1.0))
+        if not by_type:                       # nothing to compute, but coefficients are refused all the same
+            lib.check(lib.dpc_dense_orthogonal(None, 0, None, 0, ctypes.byref(s), None, 0), "dpc_dense_orthogonal")
+        for dtype, entries in by_type.items():
+            _run_orthogonal(lib, sources[0].device, dtype, entries, s)
+    return outs[0] if single else outs
+
+
+_ADJUST = {
+    "rms": lambda r, c: 0.2 * math.sqrt(max(r, c)),
+    "spectral": lambda r, c: math.sqrt(max(1.0, r / c)),
+    "none": lambda r, c: 1.0,
+}
+
+
+def _span(t):
+    return t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()
+
+
+def _check_apart(written, read):
+    """no two written tensors share memory, and no read one lies in a written one"""
+    spans = sorted([_span(t) + (True,) for t in written if t.numel()] + [_span(t) + (False,) for t in read if t.numel()])
+    end, end_written = 0, 0                   # how far the spans so far reach, and the written ones among them
+    for lo, hi, w in spans:
+        if lo < (end if w else end_written):
+            raise ValueError("weights and momenta must not share memory with each other or with the gradients")
+        end = max(end, hi)
+        if w:
+            end_written = max(end_written, hi)
+
+
+def _matrix_format(t):
+    """how a weight's storage is a matrix [shape[0], the rest]: torch.contiguous_format, torch.channels_last or None.  The order
+    of the columns does not matter to the update, only that it is the same in weight, gradient and momentum."""
+    if t.is_contiguous():
+        return torch.contiguous_format
+    if t.dim() == 4 and t.is_contiguous(memory_format=torch.channels_last):
+        return torch.channels_last
+    return None
+
+
+def muon_update(weights, grads, momenta, *, lr, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, coefficients=COEFFICIENTS,
+                eps=1e-7, adjust="rms"):
+    """One optimiser step on lists of weights, in place, all matrices in the same launches:
+
+        m <- momentum m + (1 - momentum) g;   u = (1 - momentum) g + momentum m  (nesterov), else m
+        w <- (1 - lr weight_decay) w - lr s newton_schulz(u)
+
+    with s = 0.2 sqrt(max(rows, cols)) (``adjust="rms"``: updates of the size that Adam's have), sqrt(max(1, rows / cols))
+    ("spectral") or 1 ("none").  A weight of more than two dimensions counts as [shape[0], the rest].  float32, bfloat16 or float16,
+    contiguous or channels_last; gradients of the weight's type and shape; momenta float32, laid out like their weights.  ``lr`` a
+    number, or a one-element float32 tensor on the device that is read when the work runs (a recorded step follows it)."""
+    weights, grads, momenta = list(weights), list(grads), list(momenta)
+    if not len(weights) == len(grads) == len(momenta):
+        raise ValueError("%d weights, %d gradients, %d momenta" % (len(weights), len(grads), len(momenta)))
+    if adjust not in _ADJUST:
+        raise ValueError("adjust must be one of %s, got %r" % (sorted(_ADJUST), adjust))
+    lr_tensor = lr if isinstance(lr, torch.Tensor) else None
+    lib = _library(*weights, *grads, *momenta, lr_tensor)
+    s = _steps_of(steps, coefficients, eps)
+    s.nesterov, s.momentum, s.weight_decay = 1 if nesterov else 0, float(momentum), float(weight_decay)
+    if not 0.0 <= s.momentum < 1.0:
+        raise ValueError("momentum must be in [0, 1), got %r" % (momentum,))
+    if not (s.weight_decay >= 0.0 and math.isfinite(s.weight_decay)):
+        raise ValueError("weight_decay must not be negative, got %r" % (weight_decay,))
+    if lr_tensor is not None:
+        if lr_tensor.numel() != 1 or lr_tensor.dtype != torch.float32:
+            raise ValueError("lr must be a number or a one-element float32 tensor, got %s %s" % (lr.dtype, tuple(lr.shape)))
+        s.lr_device = lr_tensor.data_ptr()
+    else:
+        s.lr = float(lr)
+        if not (s.lr >= 0.0 and math.isfinite(s.lr)):
+            raise ValueError("lr must not be negative, got %r" % (lr,))
+    by_type = {}
+    with torch.no_grad():
+        for i, (w, g, m) in enumerate(zip(weights, grads, momenta)):
+            _code(w, "a weight")
+            if w.dim() < 2:
+                raise ValueError("weight %d has shape %s: only matrices can be orthogonalised" % (i, tuple(w.shape)))
+            if g.dtype != w.dtype or g.shape != w.shape:
+                raise ValueError("gradient %d is %s %s, its weight %s %s" % (i, g.dtype, tuple(g.shape), w.dtype, tuple(w.shape)))
+            if m.dtype != torch.float32 or m.shape != w.shape:
+                raise ValueError("momentum %d must be float32 %s, got %s %s" % (i, tuple(w.shape), m.dtype, tuple(m.shape)))
+            form = _matrix_format(w)
+            if form is None or not m.is_contiguous(memory_format=form):
+                raise ValueError("weight %d and its momentum must be contiguous, or both channels_last" % i)
+            if not w.numel():
+                continue
+            g = g.detach()
+            if not g.is_contiguous(memory_format=form):
+                g = g.contiguous(memory_format=form)
+            rows = w.shape[0]
+            cols = w.numel() // rows
+            by_type.setdefault(w.dtype, []).append((g, m, w, rows, cols, _ADJUST[adjust](rows, cols)))
+        entries = [e for es in by_type.values() for e in es]
+        _check_apart([e[2] for e in entries] + [e[1] for e in entries], [e[0] for e in entries] + ([lr_tensor] if lr_tensor is not None else []))
+        if not by_type:
+            lib.check(lib.dpc_dense_orthogonal(None, 0, None, 0, ctypes.byref(s), None, 0), "dpc_dense_orthogonal")
+        for dtype, es in by_type.items():
+            _run_orthogonal(lib, weights[0].device, dtype, es, s)
