@@ -4,5 +4,6 @@
 #include "k_tile.inc"
 #include "k_product.inc"
 #include "k_orthogonal.inc"
+#include "k_narrow.inc"
 
 #include "host.inc"

@@ -14,11 +14,19 @@ typedef int v8i __attribute__((vector_size(32)));
 typedef float f4 __attribute__((vector_size(16)));
 typedef float f16v __attribute__((vector_size(64)));
 
-static inline float half_value(unsigned short b) {
+static inline float half_value_of(unsigned short b) {
   const int e = (b >> 10) & 31, m = b & 1023;
   float v = e == 31 ? (m ? NAN : INFINITY) : e ? ldexpf(1024 + m, e - 25) : ldexpf(m, -24);
   return b & 0x8000 ? -v : v;
 }
+struct Halves {
+  float of[65536];
+  Halves() {
+    for (int i = 0; i < 65536; ++i) of[i] = half_value_of((unsigned short)i);
+  }
+};
+inline const Halves g_halves;
+static inline float half_value(unsigned short b) { return g_halves.of[b]; }
 static inline unsigned half_bits(float v) {
   unsigned b;
   memcpy(&b, &v, 4);
@@ -33,11 +41,19 @@ static inline unsigned half_bits(float v) {
   const long m = lrintf(ldexpf(a, 10 - e));                   // nearest even
   return s | (unsigned)(m >= 1024 ? ((e + 15) << 10) + (m - 1024) : m);
 }
-static inline float e4m3_value(unsigned char b) {
+static inline float e4m3_value_of(unsigned char b) {
   const int e = (b >> 3) & 15, m = b & 7;
   float v = (b & 0x7f) == 0x7f ? NAN : e ? ldexpf(8 + m, e - 10) : ldexpf(m, -9);
   return b & 0x80 ? -v : v;
 }
+struct Bytes {
+  float of[256];
+  Bytes() {
+    for (int i = 0; i < 256; ++i) of[i] = e4m3_value_of((unsigned char)i);
+  }
+};
+inline const Bytes g_bytes;
+static inline float e4m3_value(unsigned char b) { return g_bytes.of[b]; }
 static inline unsigned e4m3_bits(float v) {
   unsigned b;
   memcpy(&b, &v, 4);
@@ -131,9 +147,23 @@ static inline f4 mma_f8_16(v8i a, v8i b, f4 c, int sa, int sb) {
   hipemu::wave_sync();
   return c;
 }
-static inline void load_lds16(const void* g, void* base) {
-  memcpy(static_cast<unsigned char*>(base) + 16 * (hipemu::cur().flat & 63u), g, 16);
+typedef const unsigned char* Window;
+static inline Window window(const void* p) { return static_cast<const unsigned char*>(p); }
+static inline void load_lds16(Window w, void* base, unsigned offset, unsigned line) {
+  memcpy(static_cast<unsigned char*>(base) + 16 * (hipemu::cur().flat & 63u), w + (size_t)offset + line, 16);
 }
-static inline void wait_lds_loads() {}
+template <int N>
+static inline void line_barrier() { hipemu::sync(); }
+typedef double d4 __attribute__((vector_size(32)));
+static inline d4 mma_f64(double a, double b, d4 c) {
+  static thread_local double x[1024], y[1024];
+  const unsigned f = hipemu::cur().flat, w = f & ~63u, l = f & 63u;
+  x[f] = a, y[f] = b;
+  hipemu::wave_sync();
+  for (unsigned e = 0; e < 4; ++e)
+    for (unsigned k = 0; k < 4; ++k) c[e] += x[w + l / 16 + 4 * e + 16 * k] * y[w + l % 16 + 16 * k];
+  hipemu::wave_sync();
+  return c;
+}
 static inline int uniform(int v) { return v; }
 }  // namespace dense
