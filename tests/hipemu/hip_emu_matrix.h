@@ -8,6 +8,9 @@
 
 struct uint2 { unsigned x, y; };
 
+#define DENSE_ORDER_READS(n) ((void)0)
+#define DENSE_ORDER_MATRIX(n) ((void)0)
+
 namespace dense {
 typedef int v4i __attribute__((vector_size(16)));
 typedef int v8i __attribute__((vector_size(32)));
