@@ -45,6 +45,11 @@ SIGNATURES = {
     "dpc_dense_colsum": (_I, [_P, _I, _I, _P, _I, _P]),
     "dpc_dense_product_workspace": (_Z, [_I, _I, _I, _I]),
     "dpc_dense_product": (_I, [_P, _I, _I, _I, _P, _P, _P, _P, _P, _I, _P, _I, _P, _Z]),
+    "dpc_dense_linear_sizes": (_I, [_I, _I, _I, _I, _I, _I, ctypes.POINTER(_Z)]),
+    "dpc_dense_linear_forward": (_I, [_P, _I, _I, _I, _P, _Z, _I, _P, _Z, _I, _P, _I, _P, _I, _P, _Z, _P, _Z]),
+    "dpc_dense_linear_backward": (_I, [_P, _I, _I, _I, _P, _Z, _I, _I, _I, _P, _Z, _P, _P, _P, _P, _Z]),
+    "dpc_dense_linear_serve_workspace": (_Z, [_I, _I, _I, _I]),
+    "dpc_dense_linear_serve": (_I, [_P, _I, _I, _I, _P, _Z, _I, _P, _P, _P, _I, _P, _P, _Z]),
     "dpc_dense_orthogonal_workspace": (_Z, [_I, _MP, _I]),
     "dpc_dense_orthogonal": (_I, [_P, _I, _MP, _I, _TP, _P, _Z]),
 }

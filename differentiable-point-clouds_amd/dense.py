@@ -15,7 +15,7 @@ import math
 
 import torch
 
-from . import _dense_capi, ops
+from . import _dense_capi, _dense_ext, ops
 from ._dense_capi import BLOCK, DpcDenseMatrix, DpcDenseSteps
 
 _CODES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
@@ -46,17 +46,47 @@ def _library(*tensors):
     return lib
 
 
+def _compiled():
+    """(compiled binding, id of the active library in it), or (None, None): ctypes then drives the same library"""
+    ext = _dense_ext.module()
+    if ext is None:
+        return None, None
+    lib = _dense_capi.get_library()
+    lib_id = lib.__dict__.get("_ext_id")
+    if lib_id is None:
+        lib_id = lib.__dict__["_ext_id"] = ext.open_library(lib.path, lib.host_memory)
+    return ext, lib_id
+
+
+def _raise_rc(e):
+    """a status of the library that the compiled binding passed on: raise what the ctypes binding raises"""
+    msg = str(e)
+    if msg.startswith("DPC_RC:"):
+        _, rc, what = msg.split("\n", 1)[0].split(":", 2)
+        _dense_capi.DenseLibrary.check(int(rc), what.strip())
+
+
+def _check_tensors(*ts):
+    for t in ts:
+        if not isinstance(t, torch.Tensor):
+            raise TypeError("expected a torch.Tensor, got %r" % type(t))
+
+
 def _code(t, what):
     if t.dtype not in _CODES:
         raise TypeError("%s must be float32, bfloat16 or float16, got %s" % (what, t.dtype))
     return _CODES[t.dtype]
 
 
+_HERE = contextlib.nullcontext()
+
+
 def _on(lib, device):
     """(context that makes `device` current, its current stream)"""
     if lib.host_memory:
-        return contextlib.nullcontext(), None
-    return torch.cuda.device(device), torch.cuda.current_stream(device).cuda_stream
+        return _HERE, None
+    guard = _HERE if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+    return guard, torch._C._cuda_getCurrentRawStream(device.index)
 
 
 def _bytes(n, device):
@@ -106,40 +136,24 @@ def _check_packed(w):
         raise ValueError("values and scales must be contiguous, values 16-byte aligned")
 
 
-def _quantize(lib, t, along_cols, along_rows, sums=False):
-    """t [rows, cols] in 8 bits: ((values, scales) with blocks along the columns | None, the same of the transposed matrix | None,
-    sums of each 128 rows | None)"""
-    rows, cols = t.shape
-    dev = t.device
-    nc, nr = -(-cols // BLOCK), -(-rows // BLOCK)
-    q = s = qt = st = cs = None
-    if along_cols:
-        q, s = _buffer((rows, nc * BLOCK), torch.float8_e4m3fn, dev), _buffer((nc, rows), torch.uint8, dev)
-    if along_rows:
-        qt, st = _buffer((cols, nr * BLOCK), torch.float8_e4m3fn, dev), _buffer((nr, cols), torch.uint8, dev)
-        if sums:
-            cs = _buffer((nr, cols), torch.float32, dev)
-    guard, stream = _on(lib, dev)
-    p = ops._ptr
-    with guard:
-        lib.check(lib.dpc_dense_quantize(stream, rows, cols, _CODES[t.dtype], t.data_ptr(), t.stride(0) if rows > 1 else cols, p(q), p(s),
-                                         p(qt), p(st), p(cs)), "dpc_dense_quantize")
-    return (q, s), (qt, st), cs
+_SIZES = {}
 
 
-def _product(lib, a, b, bias, dtype):
-    """[rows of a, rows of b] = a b^T (+ bias) of two 8-bit forms with blocks along the summed axis"""
-    (qa, sa), (qb, sb) = a, b
-    m, n, blocks = qa.shape[0], qb.shape[0], sa.shape[0]
-    out = _buffer((m, n), dtype, qa.device)
-    code = _CODES[dtype]
-    need = lib.dpc_dense_product_workspace(m, n, blocks, code)
-    hold, ws = _bytes(need, qa.device) if need else (None, None)
-    guard, stream = _on(lib, qa.device)
-    with guard:
-        lib.check(lib.dpc_dense_product(stream, m, n, blocks, qa.data_ptr(), sa.data_ptr(), qb.data_ptr(), sb.data_ptr(), ops._ptr(bias),
-                                        0 if bias is None else _CODES[bias.dtype], out.data_ptr(), code, ws, need), "dpc_dense_product")
-    return out
+def _sizes(lib, m, k, n, x_type, w_type, needs):
+    """bytes that a layer's passes need: (kept for the backward pass, forward workspace, backward workspace); by sizes alone"""
+    key = (id(lib), m, k, n, x_type, w_type, needs)
+    got = _SIZES.get(key)
+    if got is None:
+        out = (ctypes.c_size_t * 3)()
+        lib.check(lib.dpc_dense_linear_sizes(m, k, n, x_type, w_type, needs, out), "dpc_dense_linear_sizes")
+        if len(_SIZES) > 1024:
+            _SIZES.clear()
+        got = _SIZES[key] = tuple(out)
+    return got
+
+
+def _ld(t):
+    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
 class _LinearFp8(torch.autograd.Function):
@@ -147,33 +161,46 @@ class _LinearFp8(torch.autograd.Function):
     blocks along the axis that its product sums over: dx = Q(dy) Q(w^T)^T, dw = Q(dy^T) Q(x^T)^T, dbias = sum of dy's rows."""
 
     @staticmethod
-    def forward(ctx, x, w, bias):
-        lib = _library(x, w, bias)
-        need_x, need_w, need_b = ctx.needs_input_grad
-        xq, xt, _ = _quantize(lib, _rows(x), True, need_w)
-        wq, wt, _ = _quantize(lib, _rows(w), True, need_x)
-        ctx.meta = (w.dtype, None if bias is None else bias.dtype)
-        ctx.save_for_backward(*xt, *wt)
-        return _product(lib, xq, wq, bias, x.dtype)
+    def forward(ctx, x, w, bias, lib):
+        need = ctx.needs_input_grad
+        needs = (1 if need[0] else 0) | (2 if need[1] else 0) | (4 if need[2] else 0)
+        x, w = _rows(x), _rows(w)
+        m, k, n = x.shape[0], x.shape[1], w.shape[0]
+        x_type, w_type = _CODES[x.dtype], _CODES[w.dtype]
+        saved_bytes, forward_bytes, _ = _sizes(lib, m, k, n, x_type, w_type, needs)
+        out = _buffer((m, n), x.dtype, x.device)
+        saved, saved_at = _bytes(saved_bytes, x.device)
+        hold, ws = _bytes(forward_bytes, x.device)
+        guard, stream = _on(lib, x.device)
+        with guard:
+            rc = lib.dpc_dense_linear_forward(stream, m, k, n, x.data_ptr(), _ld(x), x_type, w.data_ptr(), _ld(w), w_type, ops._ptr(bias),
+                                              0 if bias is None else _CODES[bias.dtype], out.data_ptr(), needs, saved_at, saved_bytes, ws,
+                                              forward_bytes)
+        lib.check(rc, "dpc_dense_linear_forward")
+        ctx.save_for_backward(saved)
+        ctx.plan = (lib, m, k, n, x.dtype, w.dtype, None if bias is None else bias.dtype, needs)
+        return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        need_x, need_w, need_b = ctx.needs_input_grad
-        w_dtype, b_dtype = ctx.meta
-        xq, xs, wq, ws = ctx.saved_tensors
-        lib = _library(dy)
-        dq, dt, sums = _quantize(lib, _rows(dy), need_x, need_w or need_b, need_b)
-        dx = _product(lib, dq, (wq, ws), None, dy.dtype) if need_x else None
-        dw = _product(lib, dt, (xq, xs), None, w_dtype) if need_w else None
-        db = None
-        if need_b:
-            db = _buffer((dy.shape[1],), b_dtype, dy.device)
-            guard, stream = _on(lib, dy.device)
-            with guard:
-                lib.check(lib.dpc_dense_colsum(stream, sums.shape[0], dy.shape[1], sums.data_ptr(), _CODES[b_dtype], db.data_ptr()),
-                          "dpc_dense_colsum")
-        return dx, dw, db
+        lib, m, k, n, x_dtype, w_dtype, b_dtype, needs = ctx.plan
+        saved, = ctx.saved_tensors
+        dy = _rows(dy)
+        dev = dy.device
+        x_type, w_type = _CODES[x_dtype], _CODES[w_dtype]
+        saved_bytes, _, need = _sizes(lib, m, k, n, x_type, w_type, needs)
+        dx = _buffer((m, k), x_dtype, dev) if needs & 1 else None
+        dw = _buffer((n, k), w_dtype, dev) if needs & 2 else None
+        db = _buffer((n,), b_dtype, dev) if needs & 4 else None
+        hold, ws = _bytes(need, dev)
+        guard, stream = _on(lib, dev)
+        p = ops._ptr
+        with guard:
+            rc = lib.dpc_dense_linear_backward(stream, m, k, n, dy.data_ptr(), _ld(dy), x_type, w_type, _CODES[b_dtype] if needs & 4 else 0,
+                                               (saved.data_ptr() + 255) & ~255, saved_bytes, p(dx), p(dw), p(db), ws, need)
+        lib.check(rc, "dpc_dense_linear_backward")
+        return dx, dw, db, None
 
 
 def pack_weight_fp8(weight):
@@ -182,8 +209,15 @@ def pack_weight_fp8(weight):
     _code(weight, "weight")
     if weight.dim() != 2:
         raise ValueError("weight must be [out_features, in_features], got %s" % (tuple(weight.shape),))
-    (q, s), _, _ = _quantize(lib, _rows(weight.detach()), True, False)
-    return Fp8Weight(q, s, weight.shape[1])
+    w = _rows(weight.detach())
+    n, k = w.shape
+    blocks = -(-k // BLOCK)
+    q, s = _buffer((n, blocks * BLOCK), torch.float8_e4m3fn, w.device), _buffer((blocks, n), torch.uint8, w.device)
+    guard, stream = _on(lib, w.device)
+    with guard:
+        rc = lib.dpc_dense_quantize(stream, n, k, _CODES[w.dtype], w.data_ptr(), _ld(w), q.data_ptr(), s.data_ptr(), None, None, None)
+    lib.check(rc, "dpc_dense_quantize")
+    return Fp8Weight(q, s, k)
 
 
 def linear_fp8(x, weight, bias=None):
@@ -196,6 +230,16 @@ def linear_fp8(x, weight, bias=None):
     gradient.  A value that is not finite makes NaN of every result that it enters.  float32 magnitudes are meant to lie within
     2^-100 .. 2^100."""
     packed = isinstance(weight, Fp8Weight)
+    ext, lib_id = _compiled()
+    if ext is not None:
+        _check_tensors(x, *((weight.values, weight.scales) if packed else (weight,)), *(() if bias is None else (bias,)))
+        try:
+            if packed:
+                return ext.serve(x, weight.values, weight.scales, int(weight.in_features), bias, lib_id, bool(ops._POISON))
+            return ext.linear(x, weight, bias, lib_id, bool(ops._POISON))
+        except RuntimeError as e:
+            _raise_rc(e)
+            raise
     lib = _library(x, weight.values if packed else weight, weight.scales if packed else None, bias)
     _code(x, "x")
     if packed:
@@ -215,13 +259,23 @@ def linear_fp8(x, weight, bias=None):
         bias = bias.contiguous()
     lead = x.shape[:-1]
     rows = math.prod(lead)
-    x2 = x.reshape(rows, k)
+    x2 = x if len(lead) == 1 else x.reshape(rows, k)
     if not packed:
-        return _LinearFp8.apply(x2, weight, bias).reshape(*lead, n)
+        y = _LinearFp8.apply(x2, weight, bias, lib)
+        return y if len(lead) == 1 else y.reshape(*lead, n)
     if torch.is_grad_enabled() and (x.requires_grad or bias is not None and bias.requires_grad):
         raise ValueError("a packed weight serves only: call under torch.no_grad(), or pass the weight itself")
-    xq, _, _ = _quantize(lib, _rows(x2), True, False)
-    return _product(lib, xq, (weight.values, weight.scales), bias, x.dtype).reshape(*lead, n)
+    x2 = _rows(x2)
+    out = _buffer((rows, n), x.dtype, x.device)
+    code = _CODES[x.dtype]
+    need = lib.dpc_dense_linear_serve_workspace(rows, k, n, code)
+    hold, ws = _bytes(need, x.device) if need else (None, None)
+    guard, stream = _on(lib, x.device)
+    with guard:
+        rc = lib.dpc_dense_linear_serve(stream, rows, k, n, x2.data_ptr(), _ld(x2), code, weight.values.data_ptr(), weight.scales.data_ptr(),
+                                        ops._ptr(bias), 0 if bias is None else _CODES[bias.dtype], out.data_ptr(), ws, need)
+    lib.check(rc, "dpc_dense_linear_serve")
+    return out if len(lead) == 1 else out.reshape(*lead, n)
 
 
 class Fp8Linear(torch.nn.Linear):
@@ -234,7 +288,8 @@ class Fp8Linear(torch.nn.Linear):
 # ---------------------------------------------------------------------------
 # orthogonalisation and the update
 # ---------------------------------------------------------------------------
-def _steps_of(steps, coefficients, eps):
+def _coefficients_of(steps, coefficients, eps):
+    """a, b, c of every step in one list, after the checks"""
     if isinstance(steps, bool) or not isinstance(steps, int) or not 1 <= steps <= _dense_capi.MAX_STEPS:
         raise ValueError("steps must be a whole number in 1 .. %d, got %r" % (_dense_capi.MAX_STEPS, steps))
     if not (eps > 0 and math.isfinite(eps)):
@@ -244,10 +299,15 @@ def _steps_of(steps, coefficients, eps):
         coefficients = (coefficients,) * steps
     if len(coefficients) != steps or any(len(c) != 3 for c in coefficients):
         raise ValueError("coefficients must be (a, b, c), or one such triple for each of the %d steps" % steps)
+    return [float(v) for abc in coefficients for v in abc]
+
+
+def _steps_of(steps, coefficients, eps):
+    flat = _coefficients_of(steps, coefficients, eps)
     s = DpcDenseSteps()
     s.steps, s.eps = steps, float(eps)
-    for i, abc in enumerate(coefficients):
-        s.coefficients[i][0], s.coefficients[i][1], s.coefficients[i][2] = (float(v) for v in abc)
+    for i, v in enumerate(flat):
+        s.coefficients[i // 3][i % 3] = v
     return s
 
 
@@ -275,6 +335,16 @@ def newton_schulz(grads, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
     to its own.  ``coefficients``: (a, b, c), or a triple for each step; refused where the scalar iteration leaves (-3.5, 3.5)."""
     single = isinstance(grads, torch.Tensor)
     mats = [grads] if single else list(grads)
+    ext, lib_id = _compiled()
+    if ext is not None:
+        _check_tensors(*mats)
+        flat = _coefficients_of(steps, coefficients, eps)
+        try:
+            outs = ext.newton_schulz(mats, steps, flat, eps, single, lib_id, bool(ops._POISON))
+        except RuntimeError as e:
+            _raise_rc(e)
+            raise
+        return outs[0] if single else outs
     lib = _library(*mats)
     s = _steps_of(steps, coefficients, eps)
     for g in mats:
@@ -303,6 +373,9 @@ _ADJUST = {
     "spectral": lambda r, c: math.sqrt(max(1.0, r / c)),
     "none": lambda r, c: 1.0,
 }
+
+
+_ADJUST_CODES = {"rms": 0, "spectral": 1, "none": 2}
 
 
 def _span(t):
@@ -348,21 +421,34 @@ def muon_update(weights, grads, momenta, *, lr, momentum=0.95, nesterov=True, we
     if adjust not in _ADJUST:
         raise ValueError("adjust must be one of %s, got %r" % (sorted(_ADJUST), adjust))
     lr_tensor = lr if isinstance(lr, torch.Tensor) else None
-    lib = _library(*weights, *grads, *momenta, lr_tensor)
-    s = _steps_of(steps, coefficients, eps)
-    s.nesterov, s.momentum, s.weight_decay = 1 if nesterov else 0, float(momentum), float(weight_decay)
-    if not 0.0 <= s.momentum < 1.0:
+    momentum, weight_decay, eps = float(momentum), float(weight_decay), float(eps)
+    if not 0.0 <= momentum < 1.0:
         raise ValueError("momentum must be in [0, 1), got %r" % (momentum,))
-    if not (s.weight_decay >= 0.0 and math.isfinite(s.weight_decay)):
+    if not (weight_decay >= 0.0 and math.isfinite(weight_decay)):
         raise ValueError("weight_decay must not be negative, got %r" % (weight_decay,))
     if lr_tensor is not None:
         if lr_tensor.numel() != 1 or lr_tensor.dtype != torch.float32:
             raise ValueError("lr must be a number or a one-element float32 tensor, got %s %s" % (lr.dtype, tuple(lr.shape)))
+        lr = 0.0
+    lr = float(lr)
+    if not (lr >= 0.0 and math.isfinite(lr)):
+        raise ValueError("lr must not be negative, got %r" % (lr,))
+    ext, lib_id = _compiled()
+    if ext is not None:
+        _check_tensors(*weights, *grads, *momenta)
+        flat = _coefficients_of(steps, coefficients, eps)
+        try:
+            ext.muon_update(weights, grads, momenta, lr, lr_tensor, momentum, bool(nesterov), weight_decay, steps, flat, eps,
+                            _ADJUST_CODES[adjust], lib_id, bool(ops._POISON))
+        except RuntimeError as e:
+            _raise_rc(e)
+            raise
+        return
+    lib = _library(*weights, *grads, *momenta, lr_tensor)
+    s = _steps_of(steps, coefficients, eps)
+    s.nesterov, s.momentum, s.weight_decay, s.lr = 1 if nesterov else 0, momentum, weight_decay, lr
+    if lr_tensor is not None:
         s.lr_device = lr_tensor.data_ptr()
-    else:
-        s.lr = float(lr)
-        if not (s.lr >= 0.0 and math.isfinite(s.lr)):
-            raise ValueError("lr must not be negative, got %r" % (lr,))
     by_type = {}
     with torch.no_grad():
         for i, (w, g, m) in enumerate(zip(weights, grads, momenta)):

@@ -58,6 +58,23 @@ int dpc_dense_product(dpc_dense_stream_t stream, int M, int N, int blocks, const
                       const uint8_t* sb, const void* bias, int bias_dtype, void* out, int dtype, void* workspace,
                       size_t workspace_bytes);
 
+/* A layer's passes in one call each: out [M, N] = Q(x) Q(w)^T (+ bias) of x [M, K], w [N, K], and its gradients, those of the held values'
+ * product with dy held in 8 bits along the axis that each sums over: dx = Q(dy) Q(w^T)^T (of x_type), dw = Q(dy^T) Q(x^T)^T (of w_type),
+ * db = the sums of dy's columns (of bias_type).  needs: 1 dx, 2 dw, 4 db, the same in all three calls (in the backward call: which of
+ * dx, dw, db are not null).  sizes[3]: bytes of `saved` (what the forward call leaves for the backward one), of the forward and of the
+ * backward workspace; all 256-byte aligned.  M, K, N: at most 128 * 65535. */
+int dpc_dense_linear_sizes(int M, int K, int N, int x_type, int w_type, int needs, size_t* sizes);
+int dpc_dense_linear_forward(dpc_dense_stream_t stream, int M, int K, int N, const void* x, size_t x_ld, int x_type, const void* w, size_t w_ld,
+                             int w_type, const void* bias, int bias_type, void* out, int needs, void* saved, size_t saved_bytes,
+                             void* workspace, size_t workspace_bytes);
+int dpc_dense_linear_backward(dpc_dense_stream_t stream, int M, int K, int N, const void* dy, size_t dy_ld, int x_type, int w_type, int bias_type,
+                              const void* saved, size_t saved_bytes, void* dx, void* dw, void* db, void* workspace, size_t workspace_bytes);
+/* The same with a weight that was put into 8 bits before (q, s of dpc_dense_quantize).  Up to 16 rows take one launch that reads the weight
+ * once. */
+size_t dpc_dense_linear_serve_workspace(int M, int K, int N, int x_type);
+int dpc_dense_linear_serve(dpc_dense_stream_t stream, int M, int K, int N, const void* x, size_t x_ld, int x_type, const void* q, const uint8_t* s,
+                           const void* bias, int bias_type, void* out, void* workspace, size_t workspace_bytes);
+
 /* One matrix of dpc_dense_orthogonal, row-major, [rows, cols], no gaps between rows. */
 typedef struct DpcDenseMatrix {
   const void* grad; /* [rows, cols] of the call's dtype                                                   */

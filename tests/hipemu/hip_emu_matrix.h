@@ -110,6 +110,23 @@ static inline f16v mma_f16(v4i a, v4i b, f16v c) {
   hipemu::wave_sync();
   return c;
 }
+static inline f4 mma_f16_16(v4i a, v4i b, f4 c) {
+  Handed* h = handed();
+  const int l = (int)(hipemu::cur().flat & 63u);
+  memcpy(&h[l].a, &a, 16), memcpy(&h[l].b, &b, 16);
+  hipemu::wave_sync();
+  for (int e = 0; e < 4; ++e) {
+    double s = c[e];
+    for (int k = 0; k < 4; ++k) {
+      const unsigned short* x = reinterpret_cast<const unsigned short*>(&h[4 * (l / 16) + e + 16 * k].a);
+      const unsigned short* y = reinterpret_cast<const unsigned short*>(&h[l % 16 + 16 * k].b);
+      for (int i = 0; i < 8; ++i) s += (double)half_value(x[i]) * half_value(y[i]);
+    }
+    c[e] = (float)s;
+  }
+  hipemu::wave_sync();
+  return c;
+}
 static inline f16v mma_f8(v8i a, v8i b, f16v c, int sa, int sb) {
   Handed* h = handed();
   const int l = (int)(hipemu::cur().flat & 63u);
@@ -167,6 +184,24 @@ static inline d4 mma_f64(double a, double b, d4 c) {
     for (unsigned k = 0; k < 4; ++k) c[e] += x[w + l / 16 + 4 * e + 16 * k] * y[w + l % 16 + 16 * k];
   hipemu::wave_sync();
   return c;
+}
+static inline unsigned max_of_16(unsigned v) {
+  for (int d = 8; d >= 1; d >>= 1) {
+    float f;
+    memcpy(&f, &v, 4);
+    f = __shfl_xor(f, d);
+    unsigned w;
+    memcpy(&w, &f, 4);
+    v = v > w ? v : w;
+  }
+  return v;
+}
+static inline int __shfl(int v, int lane) {
+  float f;
+  memcpy(&f, &v, 4);
+  f = ::__shfl(f, lane);
+  memcpy(&v, &f, 4);
+  return v;
 }
 static inline int uniform(int v) { return v; }
 }  // namespace dense

@@ -21,11 +21,24 @@ def dense_emulation():
     return dpc_amd._dense_capi.DenseLibrary(os.path.join(emu_dir, "libdpc_dense_emu.so"), host_memory=True)
 
 
-@pytest.fixture(params=["emulation", pytest.param("gpu", marks=pytest.mark.gpu)])
-def device(request):
-    """where the operators run: "cpu" through the emulated kernels, or the GPU"""
+def bind(monkeypatch, binding):
+    """through the compiled binding (which has to be there: the build makes it) or through ctypes"""
+    from importlib import import_module
+    ext = import_module("differentiable-point-clouds_amd._dense_ext")
+    if binding == "ctypes":
+        monkeypatch.setattr(ext, "module", lambda: None)
+    else:
+        assert ext.module() is not None, "the compiled binding is not built: python __graft_entry__.py"
+
+
+@pytest.fixture(params=["emulation-compiled", "emulation-ctypes", pytest.param("gpu-compiled", marks=pytest.mark.gpu),
+                        pytest.param("gpu-ctypes", marks=pytest.mark.gpu)])
+def device(request, monkeypatch):
+    """where the operators run: "cpu" through the emulated kernels, or the GPU; through either binding"""
     import dpc_amd
-    lib = request.getfixturevalue("dense_emulation") if request.param == "emulation" else None
+    where, binding = request.param.split("-")
+    bind(monkeypatch, binding)
+    lib = request.getfixturevalue("dense_emulation") if where == "emulation" else None
     prev = dpc_amd._dense_capi.set_library(lib)
     yield torch.device("cpu" if lib is not None else "cuda")
     dpc_amd._dense_capi.set_library(prev)
@@ -39,9 +52,10 @@ def gpu():
     dpc_amd._dense_capi.set_library(prev)
 
 
-@pytest.fixture()
-def emulated(dense_emulation):
+@pytest.fixture(params=["compiled", "ctypes"])
+def emulated(dense_emulation, request, monkeypatch):
     import dpc_amd
+    bind(monkeypatch, request.param)
     prev = dpc_amd._dense_capi.set_library(dense_emulation)
     yield dpc_amd
     dpc_amd._dense_capi.set_library(prev)
