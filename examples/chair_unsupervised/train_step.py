@@ -42,6 +42,17 @@ def make_cfg(**kw):
     return dpc_amd.default_config(**base)
 
 
+def make_optimizer(net, kind="adam", recorded=False, fused=True):
+    """"adam": torch.optim.Adam over everything (what the reference trains with); "muon": dpc_amd.optim.Muon over the matrices --
+    updates of Adam's size, so with Adam's kind of rate -- and Adam over the rest."""
+    adam = dict(capturable=recorded, **({"fused": True} if fused else {}))
+    if kind == "adam":
+        return torch.optim.Adam(net.parameters(), lr=1e-4, **adam)
+    if kind == "muon":
+        return dpc_amd.optim.muon_with_adam(net, lr=1e-3, adam_lr=1e-4, adam=adam)
+    raise ValueError("optimizer must be 'adam' or 'muon', got %r" % (kind,))
+
+
 def synthetic_batch(cfg, device, image_size, seed):
     g = torch.Generator(device="cpu").manual_seed(seed)
     n = cfg.batch_size * cfg.step_size
@@ -91,6 +102,10 @@ def main():
                     help="record the whole step (nets, projector, loss, backward, Adam) into one HIP graph and replay it; "
                          "the schedules and the dropout draw keep moving (ModelPointCloud.enable_graph_replay).  With "
                          "--gpus N the gradient all-reduce is part of the recorded step (GradBuckets instead of DDP).")
+    ap.add_argument("--dense", default="stock", choices=["stock", "fp8"],
+                    help="the large fully connected layers: torch.nn.Linear, or products in 8 bits with block scales")
+    ap.add_argument("--optimizer", default="adam", choices=["adam", "muon"],
+                    help="muon: orthogonalised momentum for the matrices, Adam for the rest")
     args = ap.parse_args()
     dd = dpc_amd.distributed
     rank, world, device = dd.init("nccl")
@@ -100,7 +115,7 @@ def main():
                    pc_point_dropout_scheduled=args.scheduled, max_number_of_steps=args.max_steps,
                    **({} if args.scheduled else {"pc_relative_sigma_end": 3.0}))
     torch.manual_seed(0)
-    net = Im2PointCloud(cfg, args.image_size).to(device)
+    net = Im2PointCloud(cfg, args.image_size, dense=args.dense).to(device)
     model, buckets = net, None
     dist_on = dd.active()          # several ranks, or a forced one-rank group (DPC_FORCE_DIST=1: the one-GPU rehearsal)
     if dist_on and args.graph:
@@ -110,7 +125,7 @@ def main():
                                                           gradient_as_bucket_view=True)
     projector = dpc_amd.model_pc.ModelPointCloud(cfg, global_step=0, device=device)
     torch.backends.cudnn.benchmark = True          # MIOpen find mode for the stock convolutions
-    opt = torch.optim.Adam(net.parameters(), lr=1e-4, capturable=args.graph, fused=True)
+    opt = make_optimizer(net, args.optimizer, recorded=args.graph)
     inputs = synthetic_batch(cfg, device, args.image_size, seed=rank)
     run = lambda: train_step(model, projector, inputs, opt, world, buckets=buckets)
     if args.graph:
@@ -146,7 +161,8 @@ def main():
                                      "graph_recordings": getattr(run, "records", 0),
                                      "taps_at_end": list(projector.effective_tap_counts()),
                                      "collectives": dd.collective_library(),
-                                     "scheduled": bool(args.scheduled)}}))
+                                     "scheduled": bool(args.scheduled), "dense": args.dense,
+                                     "optimizer": args.optimizer}}))
     dd.finalize()
 
 

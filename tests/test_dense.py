@@ -631,3 +631,90 @@ def test_same_results_every_time(gpu):
     first = gradients(dpc_amd, x, w, b, dy) + [dpc_amd.dense.newton_schulz(g)]
     for _ in range(3):
         assert all(torch.equal(p, q) for p, q in zip(first, gradients(dpc_amd, x, w, b, dy) + [dpc_amd.dense.newton_schulz(g)]))
+
+
+# ---- the training example with both --------------------------------------------------------------------------------------------------
+def example():
+    import sys
+    here = os.path.join(ROOT, "examples", "chair_unsupervised")
+    if here not in sys.path:
+        sys.path.insert(0, here)
+    import nets
+    import train_step
+    return nets, train_step
+
+
+def check_points_layer(dpc_amd, nets, ts, device, cfg, image_size, net_kw, graph=False):
+    """steps of the example with 8-bit layers and Muon: everything stays finite and moves, and the points layer's gradient is its
+    formula's"""
+    torch.manual_seed(0)
+    net = nets.Im2PointCloud(cfg, image_size=image_size, dense="fp8", **net_kw).to(device)
+    torch.manual_seed(0)
+    stock = nets.Im2PointCloud(cfg, image_size=image_size, **net_kw)
+    assert all(torch.equal(a.cpu(), b) for a, b in zip(net.state_dict().values(), stock.state_dict().values()))
+    seen = {}
+
+    def watch(module, args, y):
+        seen["x"] = args[0].detach()
+        y.register_hook(lambda g: seen.update(dy=g.detach()))
+
+    net.decoder.pts.register_forward_hook(watch)
+    proj = dpc_amd.model_pc.ModelPointCloud(cfg, global_step=0, device=device)
+    opt = ts.make_optimizer(net, "muon", recorded=graph, fused=device.type == "cuda")
+    g = torch.Generator().manual_seed(5)
+    n = cfg.batch_size * cfg.step_size
+    inputs = {"images": torch.rand(n, image_size, image_size, 3, generator=g).to(device),
+              "masks": (torch.rand(n, image_size, image_size, 1, generator=g) > 0.5).float().to(device)}
+    before = {k: v.detach().clone() for k, v in net.named_parameters()}
+    for _ in range(2):
+        loss = ts.train_step(net, proj, inputs, opt, is_training=False)
+        assert bool(torch.isfinite(loss))
+    a, b = ref.held(seen["dy"].cpu().t()), ref.held(seen["x"].cpu().t())
+    want = a @ b.t()
+    got = net.decoder.pts.weight.grad.cpu().double()
+    assert bool(((got - want).abs() <= ref.product_tolerance(a, b, want, torch.float32)).all()) and float(want.abs().max()) > 0
+    for k, v in net.named_parameters():
+        assert bool(torch.isfinite(v).all()), k
+        if k.startswith(("decoder.pts", "encoder.fc")):
+            assert not torch.equal(v, before[k]), k
+
+
+def test_training_example_in_8_bits_with_muon(emu, emulated):
+    nets, ts = example()
+    cfg = ts.make_cfg(vox_size=16, pc_gauss_kernel_size=5, pc_num_points=64, pose_predict_num_candidates=2, step_size=2, batch_size=2,
+                      pc_point_dropout=1.0)
+    check_points_layer(emulated, nets, ts, torch.device("cpu"), cfg, 32, dict(f_dim=4, fc_dim=32, z_dim=32))
+    with pytest.raises(ValueError):
+        nets.Im2PointCloud(cfg, 32, f_dim=4, fc_dim=32, z_dim=32, dense="int4")
+    with pytest.raises(ValueError):
+        ts.make_optimizer(torch.nn.Linear(2, 2), "sgd")
+
+
+@pytest.mark.gpu
+def test_training_example_in_8_bits_with_muon_on_the_gpu(gpu):
+    import dpc_amd
+    nets, ts = example()
+    cfg = ts.make_cfg(batch_size=2, pc_point_dropout=1.0, pc_num_points=2000)
+    check_points_layer(dpc_amd, nets, ts, gpu, cfg, 64, {})
+
+
+@pytest.mark.gpu
+def test_recorded_training_example_with_muon(gpu):
+    """the example's step in one graph: every replay moves the weights, and they stay finite"""
+    import dpc_amd
+    nets, ts = example()
+    cfg = ts.make_cfg(batch_size=1, step_size=2, pc_point_dropout=1.0, pc_num_points=500, vox_size=32, pc_gauss_kernel_size=11)
+    torch.manual_seed(0)
+    net = nets.Im2PointCloud(cfg, image_size=32, f_dim=4, fc_dim=64, z_dim=64, dense="fp8").to(gpu)
+    proj = dpc_amd.model_pc.ModelPointCloud(cfg, global_step=0, device=gpu)
+    opt = ts.make_optimizer(net, "muon", recorded=True)
+    inputs = ts.synthetic_batch(cfg, gpu, 32, seed=1)
+    proj.enable_graph_replay()
+    step = dpc_amd.graphs.RecordedStep(lambda: ts.train_step(net, proj, inputs, opt), device=gpu, warmup=3)
+    last = net.decoder.pts.weight.detach().clone()
+    for _ in range(3):
+        assert bool(torch.isfinite(step()))
+        torch.cuda.synchronize()
+        now = net.decoder.pts.weight.detach().clone()
+        assert bool(torch.isfinite(now).all()) and not torch.equal(now, last)
+        last = now
