@@ -49,7 +49,7 @@ def make_optimizer(net, kind="adam", recorded=False, fused=True):
     if kind == "adam":
         return torch.optim.Adam(net.parameters(), lr=1e-4, **adam)
     if kind == "muon":
-        return dpc_amd.optim.muon_with_adam(net, lr=1e-3, adam_lr=1e-4, adam=adam)
+        return dpc_amd.optim.muon_with_adam(net, lr=1e-4, adam_lr=1e-4, adam=adam)
     raise ValueError("optimizer must be 'adam' or 'muon', got %r" % (kind,))
 
 

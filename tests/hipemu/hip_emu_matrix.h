@@ -10,6 +10,7 @@ struct uint2 { unsigned x, y; };
 
 #define DENSE_ORDER_READS(n) ((void)0)
 #define DENSE_ORDER_MATRIX(n) ((void)0)
+#define DENSE_KEEP_READS() ((void)0)
 
 namespace dense {
 typedef int v4i __attribute__((vector_size(16)));
@@ -172,6 +173,7 @@ static inline Window window(const void* p) { return static_cast<const unsigned c
 static inline void load_lds16(Window w, void* base, unsigned offset, unsigned line) {
   memcpy(static_cast<unsigned char*>(base) + 16 * (hipemu::cur().flat & 63u), w + (size_t)offset + line, 16);
 }
+static inline int load_byte(Window w, unsigned offset) { return w[offset]; }
 template <int N>
 static inline void line_barrier() { hipemu::sync(); }
 typedef double d4 __attribute__((vector_size(32)));
