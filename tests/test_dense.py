@@ -621,6 +621,18 @@ def test_other_streams_and_two_calls_at_once(gpu):
             y = dpc_amd.dense.linear_fp8(x, w)
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want[0])) and torch.equal(y, want[1])
+    # a backward pass runs on its forward pass' stream, behind what that stream still has to do
+    xf, wf, dy = draw((300, 2000), 3, torch.float32, gpu), draw((700, 2000), 4, torch.float32, gpu), draw((300, 700), 5, torch.float32, gpu)
+    want = gradients(dpc_amd, xf, wf, None, dy)
+    late, big = torch.zeros_like(xf), torch.randn(4096, 4096, device=gpu)
+    torch.cuda.synchronize()
+    with torch.cuda.stream(streams[0]):
+        for _ in range(20):
+            big = big @ big * 1e-3
+        late.copy_(xf)
+        got = gradients(dpc_amd, late, wf, None, dy)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
 
 
 @pytest.mark.gpu
