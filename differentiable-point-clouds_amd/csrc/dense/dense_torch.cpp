@@ -6,6 +6,7 @@
 // Built by __graft_entry__.build() with torch.utils.cpp_extension (host compiler only) into csrc/dense/build_torch/.
 #include <torch/extension.h>
 
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <dlfcn.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -131,6 +132,15 @@ int dim_of(int64_t n) {
   TORCH_CHECK_VALUE(n <= 0x7fffffff, "an axis of ", n, " is too long");
   return (int)n;
 }
+// While a stream records a graph: a leaf whose earlier, eager autograd graph still lives would make the recorded backward pass wait for that
+// graph's stream, which ends the process.  Refused here, where it can still be said.
+void check_recording(const Api& api, const Tensor& t) {
+  if (api.host_memory || !t.requires_grad() || t.grad_fn() || c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+  const auto leaf = torch::autograd::impl::try_get_grad_accumulator(t);
+  TORCH_CHECK(!leaf || !leaf->stream().has_value() || leaf->stream()->id() == c10::hip::getCurrentHIPStream(t.device().index()).id(),
+              "linear_fp8 is being recorded into a graph while the autograd graph of an earlier eager call of the same leaf lives: drop what keeps "
+              "it (an output, a loss) before the recording");
+}
 const void* ptr(const optional<Tensor>& t) { return t.has_value() ? t->data_ptr() : nullptr; }
 
 // ---- the product ------------------------------------------------------------------------------------------------------------------
@@ -150,10 +160,13 @@ struct LinearFp8 : public torch::autograd::Function<LinearFp8> {
                          (int)needs, saved.at, saved.n, ws.at, ws.n),
              "dpc_dense_linear_forward");
     if (needs != 0) {
-      ctx->save_for_backward({saved.hold.defined() ? saved.hold : at::empty({0}, x.options().dtype(at::kByte).requires_grad(false))});
+      Tensor keep = saved.hold;
+      if (!keep.defined()) keep = at::empty({0}, x.options().dtype(at::kByte).requires_grad(false));
+      ctx->save_for_backward({keep});
       ctx->saved_data["sizes"] = std::vector<int64_t>{lib, m, k, n, (int64_t)x.scalar_type(), (int64_t)w.scalar_type(),
                                                       bias.has_value() ? (int64_t)bias->scalar_type() : -1, needs, poison ? 1 : 0,
-                                                      (int64_t)sizes[0], (int64_t)sizes[2]};
+                                                      (int64_t)sizes[0], (int64_t)sizes[2],
+                                                      (int64_t)((uintptr_t)saved.at - (saved.n > 0 ? (uintptr_t)saved.hold.data_ptr() : 0))};
     }
     return out;
   }
@@ -164,7 +177,7 @@ struct LinearFp8 : public torch::autograd::Function<LinearFp8> {
     const int m = (int)s[1], k = (int)s[2], n = (int)s[3], needs = (int)s[7];
     const auto xt = (at::ScalarType)s[4], wt = (at::ScalarType)s[5];
     const bool poison = s[8] != 0;
-    const Tensor saved = ctx->get_saved_variables()[0];
+    Tensor saved = ctx->get_saved_variables()[0];
     variable_list out(6);
     const bool again = at::GradMode::is_enabled() && grads[0].requires_grad();
     {
@@ -176,8 +189,17 @@ struct LinearFp8 : public torch::autograd::Function<LinearFp8> {
       if (needs & 4) out[2] = buffer({n}, dy, (at::ScalarType)s[6], poison);
       const Bytes ws = bytes((size_t)s[10], dy, poison);
       const auto p = [](const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; };
+      const void* kept = nullptr;
+      if (s[9] > 0) {            // (hooks on saved tensors may have brought it back at another address)
+        kept = static_cast<const char*>(saved.data_ptr()) + s[11];
+        if ((uintptr_t)kept % 256 != 0) {
+          const Bytes again_at = bytes((size_t)s[9], dy, false);
+          at::from_blob(again_at.at, {s[9]}, again_at.hold.options()).copy_(saved.narrow(0, s[11], s[9]));
+          saved = again_at.hold, kept = again_at.at;
+        }
+      }
       check_rc(api.backward(stream_of(api, dy), m, k, n, dy.data_ptr(), ld_of(dy), code_of(dy, "dy"), wt == at::kFloat ? DPC_DENSE_F32 : wt == at::kHalf ? DPC_DENSE_F16 : DPC_DENSE_BF16,
-                            out[2].defined() ? code_of(out[2], "bias") : 0, s[9] > 0 ? aligned(saved) : nullptr, (size_t)s[9], p(out[0]), p(out[1]), p(out[2]), ws.at, ws.n),
+                            out[2].defined() ? code_of(out[2], "bias") : 0, kept, (size_t)s[9], p(out[0]), p(out[1]), p(out[2]), ws.at, ws.n),
                "dpc_dense_linear_backward");
     }
     if (again) {                 // differentiable once: a second differentiation says so
@@ -209,6 +231,11 @@ Tensor linear(const Tensor& x, const Tensor& w, const optional<Tensor>& bias_, i
     bias = bias->contiguous();
   }
   const bool grad = at::GradMode::is_enabled();
+  if (grad) {
+    check_recording(api, x);
+    check_recording(api, w);
+    if (bias.has_value()) check_recording(api, *bias);
+  }
   const int64_t needs = grad ? (x.requires_grad() ? 1 : 0) | (w.requires_grad() ? 2 : 0) | (bias.has_value() && bias->requires_grad() ? 4 : 0) : 0;
   if (x.dim() == 2) return LinearFp8::apply(x, w, bias, lib, needs, poison);
   int64_t rows = 1;
@@ -379,6 +406,10 @@ void muon_update(const std::vector<Tensor>& weights, const std::vector<Tensor>& 
     TORCH_CHECK_VALUE(p.lo >= (p.written ? end : end_written), "weights and momenta must not share memory with each other or with the gradients");
     end = std::max(end, p.hi);
     if (p.written) end_written = std::max(end_written, p.hi);
+  }
+  for (const Entry& e : all) {   // autograd graphs that hold the old weights are told
+    e.out.unsafeGetTensorImpl()->bump_version();
+    e.momentum.unsafeGetTensorImpl()->bump_version();
   }
   run_orthogonal(api, all, s, poison);
 }

@@ -152,6 +152,14 @@ def _sizes(lib, m, k, n, x_type, w_type, needs):
     return got
 
 
+def _dims(*sizes):
+    """sizes as the library's 32-bit numbers"""
+    for n in sizes:
+        if n > 0x7fffffff:
+            raise ValueError("an axis of %d is too long" % n)
+    return sizes
+
+
 def _ld(t):
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
@@ -165,7 +173,7 @@ class _LinearFp8(torch.autograd.Function):
         need = ctx.needs_input_grad
         needs = (1 if need[0] else 0) | (2 if need[1] else 0) | (4 if need[2] else 0)
         x, w = _rows(x), _rows(w)
-        m, k, n = x.shape[0], x.shape[1], w.shape[0]
+        m, k, n = _dims(x.shape[0], x.shape[1], w.shape[0])
         x_type, w_type = _CODES[x.dtype], _CODES[w.dtype]
         saved_bytes, forward_bytes, _ = _sizes(lib, m, k, n, x_type, w_type, needs)
         out = _buffer((m, n), x.dtype, x.device)
@@ -178,13 +186,13 @@ class _LinearFp8(torch.autograd.Function):
                                               forward_bytes)
         lib.check(rc, "dpc_dense_linear_forward")
         ctx.save_for_backward(saved)
-        ctx.plan = (lib, m, k, n, x.dtype, w.dtype, None if bias is None else bias.dtype, needs)
+        ctx.plan = (lib, m, k, n, x.dtype, w.dtype, None if bias is None else bias.dtype, needs, saved_at - saved.data_ptr())
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        lib, m, k, n, x_dtype, w_dtype, b_dtype, needs = ctx.plan
+        lib, m, k, n, x_dtype, w_dtype, b_dtype, needs, offset = ctx.plan
         saved, = ctx.saved_tensors
         dy = _rows(dy)
         dev = dy.device
@@ -193,12 +201,16 @@ class _LinearFp8(torch.autograd.Function):
         dx = _buffer((m, k), x_dtype, dev) if needs & 1 else None
         dw = _buffer((n, k), w_dtype, dev) if needs & 2 else None
         db = _buffer((n,), b_dtype, dev) if needs & 4 else None
+        saved_at = saved.data_ptr() + offset
+        if saved_at % 256:                       # hooks on saved tensors may have brought it back at another address
+            moved, saved_at = _bytes(saved_bytes, dev)
+            moved[saved_at - moved.data_ptr():][:saved_bytes].copy_(saved[offset:offset + saved_bytes])
         hold, ws = _bytes(need, dev)
         guard, stream = _on(lib, dev)
         p = ops._ptr
         with guard:
             rc = lib.dpc_dense_linear_backward(stream, m, k, n, dy.data_ptr(), _ld(dy), x_type, w_type, _CODES[b_dtype] if needs & 4 else 0,
-                                               (saved.data_ptr() + 255) & ~255, saved_bytes, p(dx), p(dw), p(db), ws, need)
+                                               saved_at, saved_bytes, p(dx), p(dw), p(db), ws, need)
         lib.check(rc, "dpc_dense_linear_backward")
         return dx, dw, db, None
 
@@ -210,7 +222,7 @@ def pack_weight_fp8(weight):
     if weight.dim() != 2:
         raise ValueError("weight must be [out_features, in_features], got %s" % (tuple(weight.shape),))
     w = _rows(weight.detach())
-    n, k = w.shape
+    n, k = _dims(*w.shape)
     blocks = -(-k // BLOCK)
     q, s = _buffer((n, blocks * BLOCK), torch.float8_e4m3fn, w.device), _buffer((blocks, n), torch.uint8, w.device)
     guard, stream = _on(lib, w.device)
@@ -228,7 +240,7 @@ def linear_fp8(x, weight, bias=None):
     ``weight`` [out_features, in_features], float32, bfloat16 or float16 (not necessarily x's type): differentiable in x, weight
     and bias, once; the gradients' products run in 8 bits as well.  ``weight`` an ``Fp8Weight``: serving; x must not require a
     gradient.  A value that is not finite makes NaN of every result that it enters.  float32 magnitudes are meant to lie within
-    2^-100 .. 2^100."""
+    2^-100 .. 2^100.  No axis longer than 128 * 65535."""
     packed = isinstance(weight, Fp8Weight)
     ext, lib_id = _compiled()
     if ext is not None:
@@ -266,6 +278,7 @@ def linear_fp8(x, weight, bias=None):
     if torch.is_grad_enabled() and (x.requires_grad or bias is not None and bias.requires_grad):
         raise ValueError("a packed weight serves only: call under torch.no_grad(), or pass the weight itself")
     x2 = _rows(x2)
+    _dims(rows, n, k)
     out = _buffer((rows, n), x.dtype, x.device)
     code = _CODES[x.dtype]
     need = lib.dpc_dense_linear_serve_workspace(rows, k, n, code)
@@ -332,7 +345,8 @@ def newton_schulz(grads, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
 
     ``grads``: a tensor [..., rows, cols], or a list of matrices of any sizes; all of a list run in the same launches.  The result
     has the same form and type; no gradient flows.  float32 and float16 compute to single precision's accuracy, bfloat16
-    to its own.  ``coefficients``: (a, b, c), or a triple for each step; refused where the scalar iteration leaves (-3.5, 3.5)."""
+    to its own.  Sides up to 2^20, the shorter one up to 16384.  ``coefficients``: (a, b, c), or a triple for each step; refused where
+    the scalar iteration leaves (-3.5, 3.5)."""
     single = isinstance(grads, torch.Tensor)
     mats = [grads] if single else list(grads)
     ext, lib_id = _compiled()
@@ -358,7 +372,7 @@ def newton_schulz(grads, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
         for g, o in zip(sources, outs):
             if not g.numel():
                 continue
-            rows, cols = g.shape[-2:]
+            rows, cols = _dims(*g.shape[-2:])
             for a, b in zip(g.reshape(-1, rows, cols).unbind(0), o.view(-1, rows, cols).unbind(0)):
                 by_type.setdefault(g.dtype, []).append((a, None, b, rows, cols, 1.0))
         if not by_type:                       # nothing to compute, but coefficients are refused all the same
@@ -469,10 +483,12 @@ def muon_update(weights, grads, momenta, *, lr, momentum=0.95, nesterov=True, we
                 g = g.contiguous(memory_format=form)
             rows = w.shape[0]
             cols = w.numel() // rows
+            _dims(rows, cols)
             by_type.setdefault(w.dtype, []).append((g, m, w, rows, cols, _ADJUST[adjust](rows, cols)))
         entries = [e for es in by_type.values() for e in es]
         _check_apart([e[2] for e in entries] + [e[1] for e in entries], [e[0] for e in entries] + ([lr_tensor] if lr_tensor is not None else []))
         if not by_type:
             lib.check(lib.dpc_dense_orthogonal(None, 0, None, 0, ctypes.byref(s), None, 0), "dpc_dense_orthogonal")
+        torch.autograd.graph.increment_version([e[i] for e in entries for i in (1, 2)])   # autograd graphs that hold the old weights are told
         for dtype, es in by_type.items():
             _run_orthogonal(lib, weights[0].device, dtype, es, s)

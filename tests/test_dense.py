@@ -240,6 +240,21 @@ def test_fp8_linear_module(device):
     assert sorted(layer.state_dict()) == ["bias", "weight"]
 
 
+@pytest.mark.parametrize("offset", [0, 16, 144])
+def test_product_kept_forms_may_be_moved(device, offset):
+    """hooks on saved tensors (offloading) bring back what the forward pass kept at another address"""
+    import dpc_amd
+    x, w, dy = draw((130, 200), 1, torch.float32, device), draw((70, 200), 2, torch.float32, device), draw((130, 70), 3, torch.float32, device)
+    want = gradients(dpc_amd, x, w, None, dy)
+
+    def move(t):
+        there = torch.empty(t.numel() + 256, dtype=t.dtype, device=t.device)[offset:offset + t.numel()]
+        return there.copy_(t)
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.cpu(), lambda t: move(t.to(device))):
+        got = gradients(dpc_amd, x, w, None, dy)
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_product_refusals(emulated):
     d = emulated.dense
     x, w = torch.ones(2, 8), torch.ones(3, 8)
@@ -417,6 +432,18 @@ def test_muon_update_of_filters_in_both_layouts(device):
         assert ref.off(got, flat[0]) <= 2 * ref.orthogonal_tolerance(torch.float32)
 
 
+def test_muon_update_is_seen_by_autograd(device):
+    """a graph that holds the weights as they were refuses its backward pass after the update, as after any change in place"""
+    import dpc_amd
+    w = draw((8, 12), 1, torch.float32, device).requires_grad_()
+    x = draw((3, 12), 2, torch.float32, device).requires_grad_()
+    y = x @ w.t()
+    dpc_amd.dense.muon_update([w], [torch.ones_like(w)], [torch.zeros(8, 12, device=device)], lr=0.1)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+    (x @ w.t()).sum().backward()
+
+
 def test_muon_update_refusals(emulated):
     up = emulated.dense.muon_update
     w, g, m = torch.ones(3, 4), torch.ones(3, 4), torch.zeros(3, 4)
@@ -459,6 +486,14 @@ def test_refusals_by_the_library_itself(dense_emulation):
     assert lib.dpc_dense_quantize(None, 1, 4, 0, a, 4, None, None, None, None, None) == -1
     assert lib.dpc_dense_quantize(None, 1, 4, 0, a, 4, a, a, None, None, a) == -1
     assert lib.dpc_dense_quantize(None, 1, 4, 0, a, 4, a + 1, a, None, None, None) == -4
+    for far in (0x7fffffff, 0x7fffffff - 128):
+        assert lib.dpc_dense_quantize(None, 1, far, 0, a, far, a, a, None, None, None) == -2
+        assert lib.dpc_dense_quantize(None, far, 1, 0, a, 1, None, None, a, a, None) == -2
+        assert lib.dpc_dense_colsum(None, 1, far, a, 0, a) == -2
+        assert lib.dpc_dense_product(None, far, 1, 1, a, a, a, a, None, 0, a, 0, None, 0) == -2
+        assert lib.dpc_dense_product(None, 1, far, 1, a, a, a, a, None, 0, a, 0, None, 0) == -2
+    assert lib.dpc_dense_product(None, 1, 1, 65536, a, a, a, a, None, 0, a, 0, None, 0) == -2
+    assert lib.dpc_dense_linear_serve(None, 1, 128 * 65535 + 1, 1, a, 1 << 30, 0, a, a, None, 0, a, None, 0) == -2
     assert lib.dpc_dense_colsum(None, 1, 4, None, 0, a) == -1
     assert lib.dpc_dense_product(None, 1, 1, 1, a, a, a, a, None, 0, None, 0, None, 0) == -1
     assert lib.dpc_dense_product(None, 1, 1, 1, a, a, a, a, a, 7, a, 0, None, 0) == -3
@@ -602,6 +637,35 @@ def test_recorded_steps_equal_eager_ones(gpu):
         runs.append((losses, [p.detach().clone() for net in nets for p in net.parameters()]))
     for a, b in zip(runs[0][0] + runs[0][1], runs[1][0] + runs[1][1]):
         assert torch.equal(a, b)
+
+
+@pytest.mark.gpu
+def test_recording_beside_a_living_eager_graph_is_refused(gpu):
+    """the recorded backward pass would wait for the eager graph's stream; refused before anything is enqueued, and fine once it is gone"""
+    import dpc_amd
+    x, w, dy = (draw(s, i, torch.float32, gpu) for i, s in enumerate(((5, 24), (70, 24), (5, 70))))
+    w.requires_grad_()
+    eager = dpc_amd.dense.linear_fp8(x, w)
+    want, = torch.autograd.grad(eager, w, dy, retain_graph=True)
+    torch.cuda.synchronize()
+    refused = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(refused):
+        with pytest.raises(RuntimeError, match="earlier eager call of the same leaf"):
+            dpc_amd.dense.linear_fp8(x, w)
+        with torch.no_grad():
+            z = dpc_amd.dense.linear_fp8(x, w)               # nothing to differentiate, nothing to refuse
+    refused.replay()
+    assert torch.equal(z, eager)
+    del eager
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = dpc_amd.dense.linear_fp8(x, w)
+        y2 = dpc_amd.dense.linear_fp8(x, w)                  # the leaf's graph now lives, but it is the recorded one
+        got, = torch.autograd.grad(y + 0 * y2, w, dy)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
 
 
 @pytest.mark.gpu
