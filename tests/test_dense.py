@@ -333,8 +333,10 @@ def test_newton_schulz_batches_strides_and_ends(device, dtype):
             bad = torch.ones_like(z)
             bad[2, 3] = v
             good = ref.gradient((20, 20), 0, dtype).to(device)
-            a, b = ns([bad, good])
-            assert bool(torch.isnan(a).all()) and torch.equal(b, ns(good))     # its neighbours in the list are not touched
+            a, b = ns([bad, good])                          # its neighbours in the list are not touched
+            # (beside a longer side than 64 the tiled form computes it, alone the narrow one: each is within the tolerance of the exact
+            # result, so they are within twice that of each other; where both calls take one form they are equal)
+            assert bool(torch.isnan(a).all()) and ref.off(b, ns(good)) <= (2 * ref.orthogonal_tolerance(dtype) if z is zero else 0.0)
     same = ns([batch[0], batch[0]])
     assert torch.equal(same[0], same[1])
     keep = batch.clone()
