@@ -128,10 +128,10 @@ static inline f4 mma_f16_16(v4i a, v4i b, f4 c) {
   hipemu::wave_sync();
   return c;
 }
-static inline f16v mma_f8(v8i a, v8i b, f16v c, int sa, int sb) {
+static inline f16v mma_f8(v8i a, v8i b, f16v c, int sa, int i, int sb, int j) {
   Handed* h = handed();
   const int l = (int)(hipemu::cur().flat & 63u);
-  h[l] = Handed{a, b, sa & 255, sb & 255};
+  h[l] = Handed{a, b, (sa >> (8 * i)) & 255, (sb >> (8 * j)) & 255};
   hipemu::wave_sync();
   for (int e = 0; e < 16; ++e) {
     const int row = 8 * (e / 4) + 4 * (l / 32) + e % 4, col = l % 32;
@@ -173,7 +173,9 @@ static inline Window window(const void* p) { return static_cast<const unsigned c
 static inline void load_lds16(Window w, void* base, unsigned offset, unsigned line) {
   memcpy(static_cast<unsigned char*>(base) + 16 * (hipemu::cur().flat & 63u), w + (size_t)offset + line, 16);
 }
-static inline int load_byte(Window w, unsigned offset) { return w[offset]; }
+static inline void load_lds_byte(Window w, void* base, unsigned offset) {
+  static_cast<unsigned*>(base)[hipemu::cur().flat & 63u] = w[offset];
+}
 template <int N>
 static inline void line_barrier() { hipemu::sync(); }
 typedef double d4 __attribute__((vector_size(32)));
