@@ -1,6 +1,6 @@
 // dense_torch.cpp -- compiled PyTorch binding of the dense-layer operators: what dense.py does through ctypes (checks, allocations, the
 // current stream, autograd bookkeeping), in C++, because a training step's calls are launch-bound at the sizes of the networks
-// (80 x 4096 -> 1024 with gradients: 50 us of device work, 140 us of host work from Python).  No arithmetic happens here: every
+// (80 x 4096 -> 1024 with gradients: 55 us of device work, 140 us of host work from Python, 70 from here).  No arithmetic happens here: every
 // number comes out of the library, reached through dlopen on the path that Python hands over.
 //
 // Built by __graft_entry__.build() with torch.utils.cpp_extension (host compiler only) into csrc/dense/build_torch/.
