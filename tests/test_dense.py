@@ -240,6 +240,16 @@ def test_fp8_linear_module(device):
     assert sorted(layer.state_dict()) == ["bias", "weight"]
 
 
+@pytest.mark.gpu
+def test_product_of_more_than_32_bits_of_results(gpu):
+    import dpc_amd
+    x, w = draw((70000, 200), 1, torch.bfloat16, gpu), draw((70000, 200), 2, torch.bfloat16, gpu)
+    y = dpc_amd.dense.linear_fp8(x, w)
+    assert y.numel() > 2 ** 32
+    for rows in (slice(0, 2), slice(61355, 61358), slice(69998, 70000)):
+        check_product(x[rows], w, None, y[rows])
+
+
 @pytest.mark.parametrize("offset", [0, 16, 144])
 def test_product_kept_forms_may_be_moved(device, offset):
     """hooks on saved tensors (offloading) bring back what the forward pass kept at another address"""
