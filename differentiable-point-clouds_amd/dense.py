@@ -344,8 +344,8 @@ def newton_schulz(grads, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
     is at least as wide as tall): with the default coefficients the singular values move to about 1.
 
     ``grads``: a tensor [..., rows, cols], or a list of matrices of any sizes; all of a list run in the same launches.  The result
-    has the same form and type; no gradient flows.  float32 and float16 compute to single precision's accuracy, bfloat16
-    to its own.  Sides up to 2^20, the shorter one up to 16384.  ``coefficients``: (a, b, c), or a triple for each step; refused where
+    has the same form and type; no gradient flows.  The steps compute to single precision's accuracy whatever
+    the type.  Sides up to 2^20, the shorter one up to 16384.  ``coefficients``: (a, b, c), or a triple for each step; refused where
     the scalar iteration leaves (-3.5, 3.5)."""
     single = isinstance(grads, torch.Tensor)
     mats = [grads] if single else list(grads)

@@ -100,3 +100,57 @@ def test_muon_update_of_many_steps(device, dtype):
         most = 0.02 * 0.2 * max(s) ** 0.5 * bound * (1 + 2.0 ** -5) + 2 * ref.HALF_STEP[dtype] * now.cpu().double().norm()
         assert float(torch.linalg.matrix_norm(step, 2)) <= most
         assert float(step.abs().max()) > 0
+
+
+def few_ranks_tolerance(dtype, steps):
+    """A step is off by at most 12.3 * 2^-22 of what it computes with (X and the polynomial's matrices, held in 22 bits), and the steps behind
+    enlarge that by a each, at most, where the matrix has nothing itself; singular values pass 1.21 at no step and end above 0.68.  Then the
+    result's rounding.  (That is half of bf16's for five steps, so what is held in fewer bits than 22 shows.)"""
+    a = DEFAULT[0]
+    return ref.HALF_STEP[dtype] + 12.3 * 2.0 ** -22 * (a ** steps - 1) / (a - 1) * 1.21 / 0.68
+
+
+FEW_RANKS = [((70, 200), 1, 5), ((80, 90), 5, 5), ((80, 90), 5, 6), ((80, 90), 5, 8), ((130, 300), 4, 5)]
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+@pytest.mark.parametrize("shape,rank,steps", FEW_RANKS + [pytest.param(s, r, n, marks=pytest.mark.gpu) for s, r, n in (
+    ((300, 320), 8, 5), ((300, 320), 32, 5), ((320, 300), 1, 3), ((512, 640), 16, 5), ((700, 701), 16, 6), ((128, 8000), 4, 5), ((24000, 256), 16, 5))],
+    ids=lambda v: "x".join(map(str, v)) if isinstance(v, tuple) else str(v))
+def test_matrices_of_few_ranks(device, shape, rank, steps, dtype):
+    """a small batch's gradient: as exact as its type's rounding in every type, whatever the rank"""
+    if device.type == "cpu" and (shape, rank, steps) not in FEW_RANKS:
+        pytest.skip("sizes for the GPU")
+    import dpc_amd
+    g = of_rank(shape, rank, 5, dtype)
+    o = dpc_amd.dense.newton_schulz(g.to(device), steps=steps)
+    assert ref.off(o.cpu(), ref.newton_schulz(g.to(device), steps).cpu()) <= few_ranks_tolerance(dtype, steps)
+
+
+@pytest.mark.parametrize("dtype", TYPES, ids=IDS)
+def test_strong_directions(device, dtype):
+    """a few directions 64 and 256 times as strong as the rest"""
+    import dpc_amd
+    for shape, n, size in (((70, 130), 4, 64.0),) if device.type == "cpu" else (((128, 400), 4, 64.0), ((300, 320), 16, 256.0)):
+        g = torch.Generator().manual_seed(3)
+        x = torch.randn(shape, generator=g) + size / n ** 0.5 * torch.randn(shape[0], n, generator=g) @ torch.randn(n, shape[1], generator=g)
+        x = x.mul(1e-4).to(dtype)
+        assert ref.off(dpc_amd.dense.newton_schulz(x.to(device)).cpu(), ref.newton_schulz(x)) <= few_ranks_tolerance(dtype, 5)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=IDS[:2])
+def test_update_with_a_small_batchs_gradient(device, dtype):
+    """linear_fp8's gradient of 16 rows into muon_update: the weights move by the formula's step"""
+    import dpc_amd
+    n, k = (150, 70) if device.type == "cpu" else (600, 256)
+    g = torch.Generator().manual_seed(1)
+    x, dy = (torch.randn(16, s, generator=g).to(dtype).to(device) for s in (k, n))
+    w = (torch.randn(n, k, generator=g) / 16).to(dtype).to(device).requires_grad_()
+    dw, = torch.autograd.grad(dpc_amd.dense.linear_fp8(x, w), w, 1e-3 * dy)
+    was, m = w.detach().cpu().double(), torch.zeros(n, k, device=device)
+    dpc_amd.dense.muon_update([w], [dw], [m], lr=0.5, adjust="none", momentum=0.5, nesterov=False)
+    u = 0.5 * dw.cpu().double()
+    o = ref.newton_schulz(u)
+    want = was - 0.5 * o
+    tol = (ref.HALF_STEP[dtype] + 2.0 ** -23) * want.norm() + 0.5 * o.norm() * (few_ranks_tolerance(dtype, 5) - ref.HALF_STEP[dtype] + 2.0 ** -23)
+    assert (w.detach().cpu().double() - want).norm() <= tol
