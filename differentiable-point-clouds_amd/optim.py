@@ -17,6 +17,9 @@ class Muon(torch.optim.Optimizer):
     the device, which a recorded step reads anew at each replay; the momenta must exist before the recording begins (one
     eager step makes them)."""
 
+    # of a group, what the update takes; schedulers keep settings of their own there (initial_lr, max_momentum)
+    _SETTINGS = ("lr", "momentum", "nesterov", "weight_decay", "steps", "coefficients", "eps", "adjust")
+
     def __init__(self, params, lr=0.02, momentum=0.95, nesterov=True, weight_decay=0.0, steps=5, coefficients=dense.COEFFICIENTS,
                  eps=1e-7, adjust="rms"):
         super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=steps,
@@ -46,7 +49,7 @@ class Muon(torch.optim.Optimizer):
                     state["momentum_buffer"] = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
                 by_device.setdefault(p.device, []).append((p, p.grad, state["momentum_buffer"]))
             for entries in by_device.values():
-                dense.muon_update(*zip(*entries), **{k: v for k, v in group.items() if k not in ("params", "param_names")})
+                dense.muon_update(*zip(*entries), **{k: group[k] for k in self._SETTINGS if k in group})
         return loss
 
     def load_state_dict(self, state_dict):
