@@ -135,7 +135,9 @@ int dim_of(int64_t n) {
 // While a stream records a graph: a leaf whose earlier, eager autograd graph still lives would make the recorded backward pass wait for that
 // graph's stream, which ends the process.  Refused here, where it can still be said.
 void check_recording(const Api& api, const Tensor& t) {
-  if (api.host_memory || !t.requires_grad() || t.grad_fn() || c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+  if (api.host_memory || !t.requires_grad() || t.grad_fn()) return;
+  c10::OptionalDeviceGuard guard(t.device());
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
   const auto leaf = torch::autograd::impl::try_get_grad_accumulator(t);
   TORCH_CHECK(!leaf || !leaf->stream().has_value() || leaf->stream()->id() == c10::hip::getCurrentHIPStream(t.device().index()).id(),
               "linear_fp8 is being recorded into a graph while the autograd graph of an earlier eager call of the same leaf lives: drop what keeps "
@@ -234,7 +236,7 @@ Tensor linear(const Tensor& x, const Tensor& w, const optional<Tensor>& bias_, i
   if (grad) {
     check_recording(api, x);
     check_recording(api, w);
-    if (bias.has_value()) check_recording(api, *bias);
+    if (bias_.has_value()) check_recording(api, *bias_);      // (as given: a copy of a strided leaf is none)
   }
   const int64_t needs = grad ? (x.requires_grad() ? 1 : 0) | (w.requires_grad() ? 2 : 0) | (bias.has_value() && bias->requires_grad() ? 4 : 0) : 0;
   if (x.dim() == 2) return LinearFp8::apply(x, w, bias, lib, needs, poison);
