@@ -160,6 +160,37 @@ def _dims(*sizes):
     return sizes
 
 
+def _recording_stream(lib, device):
+    """the current stream of the device if it records a graph, else None"""
+    if lib.host_memory:
+        return None
+    with torch.cuda.device(device):
+        return torch.cuda.current_stream().cuda_stream if torch.cuda.is_current_stream_capturing() else None
+
+
+_MADE_ON, _ASKED = "dpc_amd.dense: recorded on", "dpc_amd.dense: asked for"
+
+
+def _check_recording(lib, *tensors):
+    """While a stream records a graph: a leaf whose earlier, eager autograd graph still lives would make the recorded backward pass wait for that
+    graph's stream, which ends the process.  Refused here, where it can still be said.  That graph holds the leaf's accumulator: what is
+    written into the accumulator's metadata is still there when it is asked for again.  One that lives is let pass if a call of this recording
+    made it; returns the accumulators, which have to live until the leaves are used."""
+    leaves = [t for t in tensors if t is not None and t.requires_grad and t.grad_fn is None]
+    stream = _recording_stream(lib, leaves[0].device) if leaves and torch.is_grad_enabled() else None
+    held = []
+    for t in leaves if stream is not None else ():
+        accumulator = lambda: torch.autograd.graph.get_gradient_edge(t).node
+        if accumulator().metadata.get(_MADE_ON) != stream:
+            accumulator().metadata[_ASKED] = True
+            if _ASKED in accumulator().metadata:
+                raise RuntimeError("linear_fp8 is being recorded into a graph while the autograd graph of an earlier eager call of the same leaf "
+                                   "lives: drop what keeps it (an output, a loss) before the recording")
+        held.append(accumulator())
+        held[-1].metadata[_MADE_ON] = stream
+    return held
+
+
 def _ld(t):
     return t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
@@ -268,6 +299,8 @@ def linear_fp8(x, weight, bias=None):
         _code(bias, "bias")
         if tuple(bias.shape) != (n,):
             raise ValueError("bias must be [%d], got %s" % (n, tuple(bias.shape)))
+    held = None if packed else _check_recording(lib, x, weight, bias)      # noqa: F841 (lives until the leaves are used)
+    if bias is not None:
         bias = bias.contiguous()
     lead = x.shape[:-1]
     rows = math.prod(lead)

@@ -1,12 +1,12 @@
-"""Recording dpc_amd.dense.linear_fp8 into a graph beside a living eager autograd graph of the same leaf is refused, whatever the
-leaf's strides."""
+"""Recording dpc_amd.dense.linear_fp8 into a graph beside a living eager autograd graph of the same leaf is refused by both bindings; the
+ctypes binding's question is tried on the CPU with a stream that only pretends to record."""
 import pytest
 import torch
 
-from test_dense import bind, draw
+from test_dense import bind, draw, emulated, dense_emulation  # noqa: F401  (fixtures)
 
 
-@pytest.fixture(params=["compiled"])
+@pytest.fixture(params=["compiled", "ctypes"])
 def gpu(request, monkeypatch):
     import dpc_amd
     bind(monkeypatch, request.param)
@@ -15,8 +15,44 @@ def gpu(request, monkeypatch):
     dpc_amd._dense_capi.set_library(prev)
 
 
+def test_a_living_graph_is_seen_through_its_accumulator(dense_emulation, monkeypatch):
+    import dpc_amd
+    bind(monkeypatch, "ctypes")
+    prev = dpc_amd._dense_capi.set_library(dense_emulation)
+    try:
+        dense = dpc_amd.dense
+        x, w, bias = draw((5, 24), 1, torch.float32, "cpu"), draw((7, 24), 2, torch.float32, "cpu"), draw((14,), 3, torch.float32, "cpu")[::2]
+        for t in (x, w, bias):
+            t.requires_grad_()
+        call = lambda: dense.linear_fp8(x, w, bias)
+        want = call().detach()
+        stream = [None]
+        monkeypatch.setattr(dense, "_recording_stream", lambda lib, device: stream[0], raising=False)
+        for alive in (lambda: call(), lambda: w * 2, lambda: bias.sum(), lambda: torch.nn.functional.linear(x, w)):
+            stream[0] = None
+            eager = alive()
+            stream[0] = 7
+            for _ in range(2):                                   # asking leaves nothing behind that would let the next call pass
+                with pytest.raises(RuntimeError, match="earlier eager call of the same leaf"):
+                    call()
+            with torch.no_grad():
+                assert torch.equal(call(), want)
+            del eager
+            first = call()
+            second = call()                                      # the leaves' graph lives, but this recording made it
+            assert torch.equal(first, want) and torch.equal(second, want)
+            stream[0] = 9                                        # another recording, the first one's graph still alive
+            with pytest.raises(RuntimeError, match="earlier eager call of the same leaf"):
+                call()
+            del first, second
+            grads = torch.autograd.grad(call(), (x, w, bias), torch.ones(5, 7))
+            assert all(g.shape == t.shape for g, t in zip(grads, (x, w, bias)))
+    finally:
+        dpc_amd._dense_capi.set_library(prev)
+
+
 @pytest.mark.gpu
-def test_recording_beside_a_living_eager_graph_is_refused_for_strided_leaves(gpu):
+def test_recording_beside_a_living_eager_graph_is_refused_by_both_bindings(gpu):
     import dpc_amd
     x, w, dy = (draw(s, i, torch.float32, gpu) for i, s in enumerate(((5, 24), (70, 24), (5, 70))))
     bias = draw((140,), 9, torch.float32, gpu)[::2]              # a strided leaf
