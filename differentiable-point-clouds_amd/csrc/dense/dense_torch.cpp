@@ -122,8 +122,9 @@ Bytes bytes(size_t n, const Tensor& like, bool poison) {
   return b;
 }
 
-// [rows, cols] with neighbouring columns and rows that do not overlap
-Tensor rows_of(const Tensor& t) {
+// [rows, cols] with neighbouring columns and rows that do not overlap, the values as they lie in memory
+Tensor rows_of(const Tensor& t_) {
+  const Tensor t = t_.resolve_neg();
   if ((t.size(1) > 1 && t.stride(1) != 1) || (t.size(0) > 1 && t.stride(0) < t.size(1))) return t.contiguous();
   return t;
 }
@@ -230,7 +231,7 @@ Tensor linear(const Tensor& x, const Tensor& w, const optional<Tensor>& bias_, i
     check_place(api, *bias, x);
     code_of(*bias, "bias");
     TORCH_CHECK_VALUE(bias->dim() == 1 && bias->size(0) == n, "bias must be [", n, "], got ", bias->sizes());
-    bias = bias->contiguous();
+    bias = bias->resolve_neg().contiguous();
   }
   const bool grad = at::GradMode::is_enabled();
   if (grad) {
@@ -257,8 +258,8 @@ Tensor serve(const Tensor& x, const Tensor& values, const Tensor& scales, int64_
   const int64_t n = values.size(0);
   TORCH_CHECK_VALUE(scales.scalar_type() == at::kByte && scales.dim() == 2 && scales.size(0) == blocks && scales.size(1) == n,
                     "scales must be uint8 [", blocks, ", ", n, "], got ", scales.scalar_type(), " ", scales.sizes());
-  TORCH_CHECK_VALUE(values.is_contiguous() && scales.is_contiguous() && (uintptr_t)values.data_ptr() % 16 == 0,
-                    "values and scales must be contiguous, values 16-byte aligned");
+  TORCH_CHECK_VALUE(values.is_contiguous() && scales.is_contiguous() && (uintptr_t)values.data_ptr() % 16 == 0 && !values.is_neg() && !scales.is_neg(),
+                    "values and scales must be contiguous, values 16-byte aligned and no negative views");
   TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) == k, "x must be [..., ", k, "], got ", x.sizes());
   optional<Tensor> bias = bias_;
   int bt = 0;
@@ -270,7 +271,7 @@ Tensor serve(const Tensor& x, const Tensor& values, const Tensor& scales, int64_
   TORCH_CHECK_VALUE(!(at::GradMode::is_enabled() && (x.requires_grad() || (bias.has_value() && bias->requires_grad()))),
                     "a packed weight serves only: call under torch.no_grad(), or pass the weight itself");
   at::AutoGradMode off(false);
-  if (bias.has_value()) bias = bias->contiguous();
+  if (bias.has_value()) bias = bias->resolve_neg().contiguous();
   std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
   int64_t rows = 1;
   for (size_t i = 0; i + 1 < shape.size(); ++i) rows *= shape[i];
@@ -342,7 +343,7 @@ std::vector<Tensor> newton_schulz(const std::vector<Tensor>& mats, int64_t steps
     TORCH_CHECK_VALUE(batched || g.dim() == 2, "expected matrices, got ", g.sizes());
   }
   for (const Tensor& g_ : mats) {
-    const Tensor g = g_.detach().contiguous();
+    const Tensor g = g_.detach().resolve_neg().contiguous();
     outs.push_back(buffer(g.sizes(), g, g.scalar_type(), poison));
     if (g.numel() == 0) continue;
     const int64_t r = g.size(-2), c = g.size(-1);
@@ -392,7 +393,9 @@ void muon_update(const std::vector<Tensor>& weights, const std::vector<Tensor>& 
                       m.scalar_type(), " ", m.sizes());
     const auto form = format_of(w);
     TORCH_CHECK_VALUE(form.has_value() && m.is_contiguous(*form), "weight ", i, " and its momentum must be contiguous, or both channels_last");
+    TORCH_CHECK_VALUE(!w.is_neg() && !m.is_neg(), "weight ", i, " or its momentum is a negative view: nothing can be written through it");
     if (w.numel() == 0) continue;
+    g = g.detach().resolve_neg();
     if (!g.is_contiguous(*form)) g = g.contiguous(*form);
     const int64_t r = w.size(0), c = w.numel() / r;
     const double scale = adjust == 0 ? 0.2 * std::sqrt((double)std::max(r, c)) : adjust == 1 ? std::sqrt(std::max(1.0, (double)r / c)) : 1.0;

@@ -105,7 +105,8 @@ def _buffer(shape, dtype, device):
 
 
 def _rows(t):
-    """t [rows, cols] with neighbouring columns and rows that do not overlap"""
+    """t [rows, cols] with neighbouring columns and rows that do not overlap, its values as they lie in memory"""
+    t = t.resolve_neg()
     if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
         return t.contiguous()
     return t
@@ -132,8 +133,8 @@ def _check_packed(w):
         raise ValueError("values must be float8_e4m3fn [out_features, %d], got %s %s" % (blocks * BLOCK, w.values.dtype, tuple(w.values.shape)))
     if w.scales.dtype != torch.uint8 or tuple(w.scales.shape) != (blocks, w.values.shape[0]):
         raise ValueError("scales must be uint8 [%d, %d], got %s %s" % (blocks, w.values.shape[0], w.scales.dtype, tuple(w.scales.shape)))
-    if not (w.values.is_contiguous() and w.scales.is_contiguous()) or w.values.data_ptr() % 16:
-        raise ValueError("values and scales must be contiguous, values 16-byte aligned")
+    if not (w.values.is_contiguous() and w.scales.is_contiguous()) or w.values.data_ptr() % 16 or w.values.is_neg() or w.scales.is_neg():
+        raise ValueError("values and scales must be contiguous, values 16-byte aligned and no negative views")
 
 
 _SIZES = {}
@@ -301,7 +302,7 @@ def linear_fp8(x, weight, bias=None):
             raise ValueError("bias must be [%d], got %s" % (n, tuple(bias.shape)))
     held = None if packed else _check_recording(lib, x, weight, bias)      # noqa: F841 (lives until the leaves are used)
     if bias is not None:
-        bias = bias.contiguous()
+        bias = bias.resolve_neg().contiguous()
     lead = x.shape[:-1]
     rows = math.prod(lead)
     x2 = x if len(lead) == 1 else x.reshape(rows, k)
@@ -399,7 +400,7 @@ def newton_schulz(grads, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
         if g.dim() < 2 or not single and g.dim() != 2:
             raise ValueError("expected %s, got %s" % ("[..., rows, cols]" if single else "matrices", tuple(g.shape)))
     with torch.no_grad():
-        sources = [g.detach().contiguous() for g in mats]
+        sources = [g.detach().resolve_neg().contiguous() for g in mats]
         outs = [_buffer(g.shape, g.dtype, g.device) for g in sources]
         by_type = {}
         for g, o in zip(sources, outs):
@@ -476,6 +477,8 @@ def muon_update(weights, grads, momenta, *, lr, momentum=0.95, nesterov=True, we
     if lr_tensor is not None:
         if lr_tensor.numel() != 1 or lr_tensor.dtype != torch.float32:
             raise ValueError("lr must be a number or a one-element float32 tensor, got %s %s" % (lr.dtype, tuple(lr.shape)))
+        if lr_tensor.is_neg():
+            raise ValueError("lr is a negative view: what lies in its memory is read when the work runs")
         lr = 0.0
     lr = float(lr)
     if not (lr >= 0.0 and math.isfinite(lr)):
@@ -509,9 +512,11 @@ def muon_update(weights, grads, momenta, *, lr, momentum=0.95, nesterov=True, we
             form = _matrix_format(w)
             if form is None or not m.is_contiguous(memory_format=form):
                 raise ValueError("weight %d and its momentum must be contiguous, or both channels_last" % i)
+            if w.is_neg() or m.is_neg():
+                raise ValueError("weight %d or its momentum is a negative view: nothing can be written through it" % i)
             if not w.numel():
                 continue
-            g = g.detach()
+            g = g.detach().resolve_neg()
             if not g.is_contiguous(memory_format=form):
                 g = g.contiguous(memory_format=form)
             rows = w.shape[0]
