@@ -95,6 +95,11 @@ void check_place(const Api& api, const Tensor& t, const Tensor& first) {
   TORCH_CHECK_VALUE(t.device() == first.device(), "tensors on different devices: ", first.device(), " and ", t.device());
 }
 
+// forward-mode derivatives are not computed here, and not dropped either
+void check_no_tangent(const Tensor& t) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(0).defined(), "the dense operators carry no forward-mode derivatives: pass the primal, or detach");
+}
+
 dpc_dense_stream_t stream_of(const Api& api, const Tensor& ref) {
   if (api.host_memory) return nullptr;
   return (dpc_dense_stream_t)c10::hip::getCurrentHIPStream(ref.device().index()).stream();
@@ -270,6 +275,8 @@ Tensor serve(const Tensor& x, const Tensor& values, const Tensor& scales, int64_
   }
   TORCH_CHECK_VALUE(!(at::GradMode::is_enabled() && (x.requires_grad() || (bias.has_value() && bias->requires_grad()))),
                     "a packed weight serves only: call under torch.no_grad(), or pass the weight itself");
+  check_no_tangent(x);
+  if (bias.has_value()) check_no_tangent(*bias);
   at::AutoGradMode off(false);
   if (bias.has_value()) bias = bias->resolve_neg().contiguous();
   std::vector<int64_t> shape(x.sizes().begin(), x.sizes().end());
@@ -338,6 +345,7 @@ std::vector<Tensor> newton_schulz(const std::vector<Tensor>& mats, int64_t steps
   std::vector<Entry> all;
   for (const Tensor& g : mats) {
     check_place(api, g, mats[0]);
+    check_no_tangent(g);
     code_of(g, "a matrix");
     TORCH_CHECK_VALUE(!batched || g.dim() >= 2, "expected [..., rows, cols], got ", g.sizes());
     TORCH_CHECK_VALUE(batched || g.dim() == 2, "expected matrices, got ", g.sizes());
@@ -370,6 +378,7 @@ void muon_update(const std::vector<Tensor>& weights, const std::vector<Tensor>& 
   const Tensor* first = weights.empty() ? nullptr : &weights[0];
   if (lr_tensor.has_value()) {
     check_place(api, *lr_tensor, first ? *first : *lr_tensor);
+    check_no_tangent(*lr_tensor);
     s.lr_device = static_cast<const float*>(lr_tensor->data_ptr());
   }
   std::vector<Entry> all;
@@ -384,7 +393,7 @@ void muon_update(const std::vector<Tensor>& weights, const std::vector<Tensor>& 
   for (size_t i = 0; i < weights.size(); ++i) {
     const Tensor &w = weights[i], &m = momenta[i];
     Tensor g = grads[i];
-    for (const Tensor* t : {&w, &m, static_cast<const Tensor*>(&g)}) check_place(api, *t, *first);
+    for (const Tensor* t : {&w, &m, static_cast<const Tensor*>(&g)}) check_place(api, *t, *first), check_no_tangent(*t);
     code_of(w, "a weight");
     TORCH_CHECK_VALUE(w.dim() >= 2, "weight ", i, " has shape ", w.sizes(), ": only matrices can be orthogonalised");
     TORCH_CHECK_VALUE(g.scalar_type() == w.scalar_type() && g.sizes() == w.sizes(), "gradient ", i, " is ", g.scalar_type(), " ", g.sizes(),

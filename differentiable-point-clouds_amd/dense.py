@@ -72,6 +72,13 @@ def _check_tensors(*ts):
             raise TypeError("expected a torch.Tensor, got %r" % type(t))
 
 
+def _check_no_tangent(*ts):
+    """forward-mode derivatives are not computed here, and not dropped either"""
+    for t in ts:
+        if t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None:
+            raise NotImplementedError("the dense operators carry no forward-mode derivatives: pass the primal, or detach")
+
+
 def _code(t, what):
     if t.dtype not in _CODES:
         raise TypeError("%s must be float32, bfloat16 or float16, got %s" % (what, t.dtype))
@@ -250,6 +257,7 @@ class _LinearFp8(torch.autograd.Function):
 def pack_weight_fp8(weight):
     """The 8-bit form of ``weight`` [out_features, in_features], to be kept for calls of ``linear_fp8``."""
     lib = _library(weight)
+    _check_no_tangent(weight)
     _code(weight, "weight")
     if weight.dim() != 2:
         raise ValueError("weight must be [out_features, in_features], got %s" % (tuple(weight.shape),))
@@ -311,6 +319,7 @@ def linear_fp8(x, weight, bias=None):
         return y if len(lead) == 1 else y.reshape(*lead, n)
     if torch.is_grad_enabled() and (x.requires_grad or bias is not None and bias.requires_grad):
         raise ValueError("a packed weight serves only: call under torch.no_grad(), or pass the weight itself")
+    _check_no_tangent(x, bias)
     x2 = _rows(x2)
     _dims(rows, n, k)
     out = _buffer((rows, n), x.dtype, x.device)
@@ -394,6 +403,7 @@ def newton_schulz(grads, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
             raise
         return outs[0] if single else outs
     lib = _library(*mats)
+    _check_no_tangent(*mats)
     s = _steps_of(steps, coefficients, eps)
     for g in mats:
         _code(g, "a matrix")
@@ -495,6 +505,7 @@ def muon_update(weights, grads, momenta, *, lr, momentum=0.95, nesterov=True, we
             raise
         return
     lib = _library(*weights, *grads, *momenta, lr_tensor)
+    _check_no_tangent(*weights, *grads, *momenta, lr_tensor)
     s = _steps_of(steps, coefficients, eps)
     s.nesterov, s.momentum, s.weight_decay, s.lr = 1 if nesterov else 0, momentum, weight_decay, lr
     if lr_tensor is not None:

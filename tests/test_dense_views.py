@@ -72,3 +72,26 @@ def test_packed_weights_that_are_negative_views_are_refused(emulated):
         pytest.skip("this torch makes no negative views of 8-bit types")
     with pytest.raises(ValueError):
         d.linear_fp8(torch.ones(2, 8), p._replace(values=values))
+
+
+def test_forward_mode_derivatives_are_refused(device):
+    """the tangent of a dual tensor is not dropped in silence, with gradients enabled or not"""
+    import dpc_amd
+    import torch.autograd.forward_ad as fw
+    d = dpc_amd.dense
+    x, w, bias = torch.ones(2, 8, device=device), torch.ones(3, 8, device=device), torch.ones(3, device=device)
+    p, m = d.pack_weight_fp8(w), torch.zeros(3, 8, device=device)
+    with fw.dual_level():
+        dual = lambda t: fw.make_dual(t.clone(), torch.ones_like(t))
+        calls = [lambda: d.linear_fp8(dual(x), w), lambda: d.linear_fp8(x, dual(w)), lambda: d.linear_fp8(x, w, dual(bias)),
+                 lambda: d.linear_fp8(dual(x), p), lambda: d.linear_fp8(x, p, dual(bias)), lambda: d.pack_weight_fp8(dual(w)),
+                 lambda: d.newton_schulz(dual(x)), lambda: d.newton_schulz([x, dual(x)]), lambda: d.muon_update([dual(w)], [w], [m], lr=0.1),
+                 lambda: d.muon_update([w], [dual(w)], [m], lr=0.1), lambda: d.muon_update([w], [w.clone()], [dual(m)], lr=0.1),
+                 lambda: d.muon_update([w], [w.clone()], [m], lr=dual(torch.ones(1, device=device)))]
+        for call in calls:
+            with pytest.raises(RuntimeError):                  # (NotImplementedError is one)
+                call()
+            with torch.no_grad(), pytest.raises(RuntimeError):
+                call()
+        want = d.linear_fp8(x, p)                              # what has no tangent runs as ever
+    assert torch.equal(want, d.linear_fp8(x, p)) and not m.any() and torch.equal(w, torch.ones_like(w))
