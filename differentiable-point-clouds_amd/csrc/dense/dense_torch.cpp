@@ -310,31 +310,45 @@ struct Entry {
   size_t offset;              // of the matrix in grad and out, in elements
 };
 
-void run_orthogonal(const Api& api, const std::vector<Entry>& all, const DpcDenseSteps& s, bool poison) {
-  if (all.empty()) {           // nothing to compute, but coefficients are refused all the same
-    check_rc(api.orthogonal(nullptr, 0, nullptr, 0, &s, nullptr, 0), "dpc_dense_orthogonal");
-    return;
-  }
-  c10::OptionalDeviceGuard guard(all[0].out.device());
+// the library's calls for a list of matrices; everything that can be refused is refused when they are planned, before the first of them runs
+struct Call {
+  std::vector<DpcDenseMatrix> matrices;
+  int code;
+};
+struct Calls {
+  std::vector<Call> list;
+  size_t workspace = 0;       // one for all of them: they follow each other on the stream
+};
+
+Calls plan_orthogonal(const Api& api, const std::vector<Entry>& all, const DpcDenseSteps& s) {
+  check_rc(api.orthogonal(nullptr, 0, nullptr, 0, &s, nullptr, 0), "dpc_dense_orthogonal");      // (coefficients)
+  Calls calls;
   for (at::ScalarType type : {at::kFloat, at::kBFloat16, at::kHalf}) {
-    std::vector<const Entry*> mine;
-    for (const Entry& e : all)
-      if (e.out.scalar_type() == type) mine.push_back(&e);
-    for (size_t at = 0; at < mine.size(); at += DPC_DENSE_MAX_MATRICES) {
-      DpcDenseMatrix ms[DPC_DENSE_MAX_MATRICES];
-      const int n = (int)std::min<size_t>(DPC_DENSE_MAX_MATRICES, mine.size() - at);
-      const size_t width = type == at::kFloat ? 4 : 2;
-      for (int i = 0; i < n; ++i) {
-        const Entry& e = *mine[at + i];
-        ms[i] = DpcDenseMatrix{static_cast<const char*>(e.grad.data_ptr()) + e.offset * width,
-                               e.momentum.defined() ? static_cast<float*>(e.momentum.data_ptr()) : nullptr,
-                               static_cast<char*>(e.out.data_ptr()) + e.offset * width, dim_of(e.rows), dim_of(e.cols), (float)e.scale, 0};
-      }
-      const int code = code_of(mine[at]->out, "a matrix");
-      const Bytes ws = bytes(api.orthogonal_workspace(n, ms, code), mine[at]->out, poison);
-      check_rc(api.orthogonal(stream_of(api, mine[at]->out), n, ms, code, &s, ws.at, ws.n), "dpc_dense_orthogonal");
+    const size_t width = type == at::kFloat ? 4 : 2;
+    bool open = false;
+    for (const Entry& e : all) {
+      if (e.out.scalar_type() != type) continue;
+      if (!open || calls.list.back().matrices.size() == DPC_DENSE_MAX_MATRICES) calls.list.push_back(Call{{}, code_of(e.out, "a matrix")});
+      open = true;
+      calls.list.back().matrices.push_back(DpcDenseMatrix{static_cast<const char*>(e.grad.data_ptr()) + e.offset * width,
+                                                          e.momentum.defined() ? static_cast<float*>(e.momentum.data_ptr()) : nullptr,
+                                                          static_cast<char*>(e.out.data_ptr()) + e.offset * width, dim_of(e.rows), dim_of(e.cols),
+                                                          (float)e.scale, 0});
     }
   }
+  for (const Call& c : calls.list) {
+    const size_t need = api.orthogonal_workspace((int)c.matrices.size(), c.matrices.data(), c.code);
+    check_rc(need > 0 ? DPC_DENSE_OK : DPC_DENSE_E_SHAPE, "dpc_dense_orthogonal");
+    calls.workspace = std::max(calls.workspace, need);
+  }
+  return calls;
+}
+
+void run_orthogonal(const Api& api, const Calls& calls, const Tensor& first, const DpcDenseSteps& s, bool poison) {
+  c10::OptionalDeviceGuard guard(first.device());
+  const Bytes ws = bytes(calls.workspace, first, poison);
+  for (const Call& c : calls.list)
+    check_rc(api.orthogonal(stream_of(api, first), (int)c.matrices.size(), c.matrices.data(), c.code, &s, ws.at, ws.n), "dpc_dense_orthogonal");
 }
 
 std::vector<Tensor> newton_schulz(const std::vector<Tensor>& mats, int64_t steps, const std::vector<double>& coefficients, double eps, bool batched,
@@ -357,7 +371,9 @@ std::vector<Tensor> newton_schulz(const std::vector<Tensor>& mats, int64_t steps
     const int64_t r = g.size(-2), c = g.size(-1);
     for (int64_t i = 0; i < g.numel() / (r * c); ++i) all.push_back(Entry{g, Tensor(), outs.back(), r, c, 1.0, (size_t)(i * r * c)});
   }
-  run_orthogonal(api, all, steps_of(steps, coefficients, eps), poison);
+  const DpcDenseSteps s = steps_of(steps, coefficients, eps);
+  const Calls calls = plan_orthogonal(api, all, s);
+  if (!all.empty()) run_orthogonal(api, calls, all[0].out, s, poison);
   return outs;
 }
 
@@ -421,11 +437,13 @@ void muon_update(const std::vector<Tensor>& weights, const std::vector<Tensor>& 
     end = std::max(end, p.hi);
     if (p.written) end_written = std::max(end_written, p.hi);
   }
+  const Calls calls = plan_orthogonal(api, all, s);
+  if (all.empty()) return;
   for (const Entry& e : all) {   // autograd graphs that hold the old weights are told
     e.out.unsafeGetTensorImpl()->bump_version();
     e.momentum.unsafeGetTensorImpl()->bump_version();
   }
-  run_orthogonal(api, all, s, poison);
+  run_orthogonal(api, calls, all[0].out, s, poison);
 }
 
 }  // namespace

@@ -367,19 +367,31 @@ def _steps_of(steps, coefficients, eps):
     return s
 
 
-def _run_orthogonal(lib, device, dtype, entries, steps):
-    """entries: (grad, momentum | None, out, rows, cols, scale) with contiguous storage"""
+def _plan_orthogonal(lib, by_type, steps):
+    """the library's calls for by_type: {dtype: [(grad, momentum | None, out, rows, cols, scale)]}, contiguous storage; everything that can be
+    refused is refused here, before the first of them runs"""
+    lib.check(lib.dpc_dense_orthogonal(None, 0, None, 0, ctypes.byref(steps), None, 0), "dpc_dense_orthogonal")      # (coefficients)
+    calls = []
+    for dtype, entries in by_type.items():
+        for at in range(0, len(entries), _dense_capi.MAX_MATRICES):
+            part = entries[at:at + _dense_capi.MAX_MATRICES]
+            ms = (DpcDenseMatrix * len(part))()
+            for m, (g, mom, out, rows, cols, scale) in zip(ms, part):
+                m.grad, m.momentum, m.out, m.rows, m.cols, m.scale = g.data_ptr(), ops._ptr(mom), out.data_ptr(), rows, cols, scale
+            need = lib.dpc_dense_orthogonal_workspace(len(part), ms, _CODES[dtype])
+            lib.check(0 if need else -2, "dpc_dense_orthogonal")                    # (sides)
+            calls.append((len(part), ms, _CODES[dtype], need))
+    return calls
+
+
+def _run_orthogonal(lib, device, calls, steps):
+    """one workspace for all calls, which follow each other on the stream"""
+    most = max(need for _, _, _, need in calls)
+    hold, ws = _bytes(most, device)
     guard, stream = _on(lib, device)
-    code = _CODES[dtype]
-    for at in range(0, len(entries), _dense_capi.MAX_MATRICES):
-        part = entries[at:at + _dense_capi.MAX_MATRICES]
-        ms = (DpcDenseMatrix * len(part))()
-        for m, (g, mom, out, rows, cols, scale) in zip(ms, part):
-            m.grad, m.momentum, m.out, m.rows, m.cols, m.scale = g.data_ptr(), ops._ptr(mom), out.data_ptr(), rows, cols, scale
-        need = lib.dpc_dense_orthogonal_workspace(len(part), ms, code)
-        hold, ws = _bytes(need, device)
-        with guard:
-            lib.check(lib.dpc_dense_orthogonal(stream, len(part), ms, code, ctypes.byref(steps), ws, need), "dpc_dense_orthogonal")
+    with guard:
+        for count, ms, code, _ in calls:
+            lib.check(lib.dpc_dense_orthogonal(stream, count, ms, code, ctypes.byref(steps), ws, most), "dpc_dense_orthogonal")
 
 
 def newton_schulz(grads, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
@@ -419,10 +431,9 @@ def newton_schulz(grads, steps=5, coefficients=COEFFICIENTS, eps=1e-7):
             rows, cols = _dims(*g.shape[-2:])
             for a, b in zip(g.reshape(-1, rows, cols).unbind(0), o.view(-1, rows, cols).unbind(0)):
                 by_type.setdefault(g.dtype, []).append((a, None, b, rows, cols, 1.0))
-        if not by_type:                       # nothing to compute, but coefficients are refused all the same
-            lib.check(lib.dpc_dense_orthogonal(None, 0, None, 0, ctypes.byref(s), None, 0), "dpc_dense_orthogonal")
-        for dtype, entries in by_type.items():
-            _run_orthogonal(lib, sources[0].device, dtype, entries, s)
+        calls = _plan_orthogonal(lib, by_type, s)
+        if calls:
+            _run_orthogonal(lib, sources[0].device, calls, s)
     return outs[0] if single else outs
 
 
@@ -536,8 +547,8 @@ def muon_update(weights, grads, momenta, *, lr, momentum=0.95, nesterov=True, we
             by_type.setdefault(w.dtype, []).append((g, m, w, rows, cols, _ADJUST[adjust](rows, cols)))
         entries = [e for es in by_type.values() for e in es]
         _check_apart([e[2] for e in entries] + [e[1] for e in entries], [e[0] for e in entries] + ([lr_tensor] if lr_tensor is not None else []))
-        if not by_type:
-            lib.check(lib.dpc_dense_orthogonal(None, 0, None, 0, ctypes.byref(s), None, 0), "dpc_dense_orthogonal")
+        calls = _plan_orthogonal(lib, by_type, s)
+        if not calls:
+            return
         torch.autograd.graph.increment_version([e[i] for e in entries for i in (1, 2)])   # autograd graphs that hold the old weights are told
-        for dtype, es in by_type.items():
-            _run_orthogonal(lib, weights[0].device, dtype, es, s)
+        _run_orthogonal(lib, weights[0].device, calls, s)

@@ -35,3 +35,28 @@ def test_muon_under_schedulers(device, name, rate):
         scheduler.step()
         assert torch.equal(w.detach(), twin)
     assert len(set(rates)) > 1
+
+
+@pytest.mark.parametrize("binding", ["compiled", "ctypes"])
+def test_a_refused_update_moves_nothing(dense_emulation, monkeypatch, binding):  # noqa: F811
+    """a matrix that the library refuses, behind others that would run in an earlier call of it: more than 40, or of another type"""
+    import dpc_amd
+    from test_dense import bind
+    bind(monkeypatch, binding)
+    prev = dpc_amd._dense_capi.set_library(dense_emulation)
+    try:
+        long = (1, (1 << 20) + 1)
+        for count, dtype in ((1, torch.bfloat16), (40, torch.float32)):
+            w = [draw((4, 5), i, torch.float32, "cpu") for i in range(count)] + [torch.ones(long, dtype=dtype)]
+            g, m = [torch.ones_like(t) for t in w], [torch.zeros(t.shape) for t in w]
+            before, versions = [t.clone() for t in w], [t._version for t in w + m]
+            with pytest.raises(dpc_amd.DpcError):
+                dpc_amd.dense.muon_update(w, g, m, lr=0.1)
+            assert all(torch.equal(a, b) for a, b in zip(w, before)) and not any(bool(t.any()) for t in m)
+            assert [t._version for t in w + m] == versions          # graphs that hold them may still run backward
+            with pytest.raises(dpc_amd.DpcError):
+                dpc_amd.dense.newton_schulz(w)
+        dpc_amd.dense.muon_update(w[:2], g[:2], m[:2], lr=0.1)
+        assert not torch.equal(w[0], before[0])
+    finally:
+        dpc_amd._dense_capi.set_library(prev)
