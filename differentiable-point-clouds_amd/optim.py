@@ -24,10 +24,20 @@ class Muon(torch.optim.Optimizer):
                  eps=1e-7, adjust="rms"):
         super().__init__(params, dict(lr=lr, momentum=momentum, nesterov=nesterov, weight_decay=weight_decay, steps=steps,
                                       coefficients=coefficients, eps=eps, adjust=adjust))
-        for group in self.param_groups:
-            for p in group["params"]:
+
+    def add_param_group(self, param_group):
+        super().add_param_group(param_group)
+        try:
+            for p in self.param_groups[-1]["params"]:
+                dense._code(p, "a parameter")
                 if p.dim() < 2:
                     raise ValueError("Muon takes matrices; a parameter of shape %s belongs to another optimiser" % (tuple(p.shape),))
+                if dense._matrix_format(p) is None:
+                    raise ValueError("Muon takes parameters that are contiguous or channels_last, got strides %s of shape %s"
+                                     % (p.stride(), tuple(p.shape)))
+        except (TypeError, ValueError):
+            self.param_groups.pop()
+            raise
 
     @torch.no_grad()
     def step(self, closure=None):

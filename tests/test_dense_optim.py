@@ -60,3 +60,21 @@ def test_a_refused_update_moves_nothing(dense_emulation, monkeypatch, binding): 
         assert not torch.equal(w[0], before[0])
     finally:
         dpc_amd._dense_capi.set_library(prev)
+
+
+def test_parameters_that_no_step_takes_are_refused_at_once():
+    from importlib import import_module
+    Muon = import_module("differentiable-point-clouds_amd.optim").Muon
+    P = torch.nn.Parameter
+    good = P(torch.ones(4, 5))
+    bad = [P(torch.ones(5)), P(torch.ones(5, 4).t()), P(torch.ones(2, 3, 4, 4, 4).to(memory_format=torch.channels_last_3d)),
+           P(torch.ones(4, 5, dtype=torch.float64))]
+    opt = Muon([good])
+    for p in bad:
+        with pytest.raises((TypeError, ValueError)):
+            Muon([p])
+        with pytest.raises((TypeError, ValueError)):
+            opt.add_param_group({"params": [p]})
+        assert len(opt.param_groups) == 1 and opt.param_groups[0]["params"] == [good]
+    opt.add_param_group({"params": P(torch.ones(2, 3, 4, 4).to(memory_format=torch.channels_last)), "lr": 0.1})
+    assert [g["lr"] for g in opt.param_groups] == [0.02, 0.1]
