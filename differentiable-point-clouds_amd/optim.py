@@ -62,16 +62,25 @@ class Muon(torch.optim.Optimizer):
                 dense.muon_update(*zip(*entries), **{k: group[k] for k in self._SETTINGS if k in group})
         return loss
 
+    @torch.no_grad()
     def load_state_dict(self, state_dict):
+        """Momenta and rates that exist keep their memory, so that a recorded step goes on with what was loaded."""
+        momenta = {p: s["momentum_buffer"] for p, s in self.state.items() if "momentum_buffer" in s}
+        rates = [g["lr"] for g in self.param_groups]
         super().load_state_dict(state_dict)
         # the base class casts state to the parameter's type; momenta stay float32
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         params = [p for g in self.param_groups for p in g["params"]]
         for i, p in zip(ids, params):
-            saved = state_dict["state"].get(i, {}).get("momentum_buffer")
-            if saved is not None:
+            saved, kept = state_dict["state"].get(i, {}).get("momentum_buffer"), momenta.get(p)
+            if saved is None and kept is None:
+                continue
+            if kept is None:
                 kept = torch.empty_like(p, dtype=torch.float32, memory_format=torch.preserve_format)
-                self.state[p]["momentum_buffer"] = kept.copy_(saved)
+            self.state[p]["momentum_buffer"] = kept.zero_() if saved is None else kept.copy_(saved)
+        for group, rate in zip(self.param_groups, rates):
+            if isinstance(rate, torch.Tensor):
+                group["lr"] = rate.copy_(torch.as_tensor(group["lr"]).reshape(rate.shape))
 
 
 class Together(object):

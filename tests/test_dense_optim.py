@@ -78,3 +78,62 @@ def test_parameters_that_no_step_takes_are_refused_at_once():
         assert len(opt.param_groups) == 1 and opt.param_groups[0]["params"] == [good]
     opt.add_param_group({"params": P(torch.ones(2, 3, 4, 4).to(memory_format=torch.channels_last)), "lr": 0.1})
     assert [g["lr"] for g in opt.param_groups] == [0.02, 0.1]
+
+
+def test_loaded_state_takes_the_place_of_the_old(device):
+    """momenta and a rate on the device keep their memory, which a recorded step reads and writes"""
+    import dpc_amd
+    make = lambda: draw((8, 12), 1, torch.float32, device).requires_grad_()
+    w, other = make(), make()
+    lr = torch.tensor([0.02], device=device)
+    opt, fresh = dpc_amd.optim.Muon([w], lr=lr), dpc_amd.optim.Muon([other], lr=0.5)
+    untouched = fresh.state_dict()
+    for p, o in ((w, opt), (other, fresh)):
+        p.grad = draw((8, 12), 2, torch.float32, device)
+        o.step()
+    where = opt.state[w]["momentum_buffer"].data_ptr()
+    for saved, rate in ((fresh.state_dict(), 0.5), (opt.state_dict(), 0.5), (untouched, 0.5)):
+        opt.load_state_dict(saved)
+        assert opt.param_groups[0]["lr"] is lr and float(lr) == rate
+        assert opt.state[w]["momentum_buffer"].data_ptr() == where
+        want = fresh.state[other]["momentum_buffer"] if saved is not untouched else torch.zeros(8, 12, device=device)
+        assert torch.equal(opt.state[w]["momentum_buffer"], want)
+    fresh.load_state_dict(opt.state_dict())                    # a number takes the loaded rate as it comes
+    assert float(fresh.param_groups[0]["lr"]) == 0.5
+
+
+@pytest.mark.gpu
+def test_recorded_steps_go_on_with_loaded_state(monkeypatch):
+    import copy
+    import dpc_amd
+    from test_dense import bind
+    bind(monkeypatch, "compiled")
+    gpu = torch.device("cuda")
+    prev = dpc_amd._dense_capi.set_library(None)
+    try:
+        net, x = toy(dpc_amd, gpu), draw((5, 24), 1, torch.float32, gpu)
+        lr = torch.full((1,), 0.02, device=gpu)
+        opt = dpc_amd.optim.Muon([net[0].weight, net[2].weight], lr=lr)
+
+        def step():
+            opt.zero_grad()
+            loss = net(x).square().sum()
+            loss.backward()
+            opt.step()
+            return loss.detach()
+        recorded = dpc_amd.graphs.RecordedStep(step, device=gpu, warmup=3)
+        recorded()
+        torch.cuda.synchronize()
+        weights, state = copy.deepcopy(net.state_dict()), copy.deepcopy(opt.state_dict())
+        runs = []
+        for _ in range(3):
+            lr.fill_(0.7)                                      # what loading has to take back
+            net.load_state_dict(weights)
+            opt.load_state_dict(state)
+            losses = [recorded().clone() for _ in range(3)]
+            torch.cuda.synchronize()
+            runs.append(losses + [p.detach().clone() for p in net.parameters()])
+        for run in runs[1:]:
+            assert all(torch.equal(a, b) for a, b in zip(run, runs[0]))
+    finally:
+        dpc_amd._dense_capi.set_library(prev)
