@@ -278,8 +278,8 @@ def linear_fp8(x, weight, bias=None):
     (whose sums are off by 1.4e-5 of the result), float32 results the half-precision one (1e-7).
 
     ``weight`` [out_features, in_features], float32, bfloat16 or float16 (not necessarily x's type): differentiable in x, weight
-    and bias, once; the gradients' products run in 8 bits as well.  ``weight`` an ``Fp8Weight``: serving; x must not require a
-    gradient.  A value that is not finite makes NaN of every result that it enters.  float32 magnitudes are meant to lie within
+    and bias, once; the gradients' products run in 8 bits as well (forward-mode derivatives are refused, here and below).  ``weight`` an
+    ``Fp8Weight``: serving; x must not require a gradient.  A value that is not finite makes NaN of every result that it enters.  float32 magnitudes are meant to lie within
     2^-100 .. 2^100.  No axis longer than 128 * 65535."""
     packed = isinstance(weight, Fp8Weight)
     ext, lib_id = _compiled()
