@@ -50,12 +50,13 @@ def test_many_steps_of_matrices_of_few_ranks(device, steps, coefficients, dtype)
     import dpc_amd
     if device.type == "cpu" and (steps, dtype) not in ((20, torch.float32), (64, torch.bfloat16)):
         pytest.skip("an emulated work-group of a thousand threads takes seconds a step")
-    mats = [of_rank(s, rank, i, dtype).to(device) for i, s in enumerate(NARROW[:1] + NARROW[3:4] if device.type == "cpu" else NARROW)
-            for rank in ((3,) if device.type == "cpu" else (1, 3, 5, 0))]
     bound = scalar_bound(steps, coefficients)
-    for g, o in zip(mats, dpc_amd.dense.newton_schulz(mats, steps=steps, coefficients=coefficients)):
-        assert bool(torch.isfinite(o).all()), tuple(g.shape)
-        assert float(torch.linalg.matrix_norm(o.cpu().double(), 2)) <= bound * (1 + 2.0 ** -5), tuple(g.shape)
+    # (beside larger matrices sides of 33 .. 64 are tiled: the last list is a call of its own)
+    for shapes in [NARROW[:1] + NARROW[3:4]] if device.type == "cpu" else [NARROW, [(80, 90), (130, 300)]]:
+        mats = [of_rank(s, rank, i, dtype).to(device) for i, s in enumerate(shapes) for rank in ((3,) if device.type == "cpu" else (1, 3, 5, 0))]
+        for g, o in zip(mats, dpc_amd.dense.newton_schulz(mats, steps=steps, coefficients=coefficients)):
+            assert bool(torch.isfinite(o).all()), tuple(g.shape)
+            assert float(torch.linalg.matrix_norm(o.cpu().double(), 2)) <= bound * (1 + 2.0 ** -5), tuple(g.shape)
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=IDS)
@@ -154,3 +155,49 @@ def test_update_with_a_small_batchs_gradient(device, dtype):
     want = was - 0.5 * o
     tol = (ref.HALF_STEP[dtype] + 2.0 ** -23) * want.norm() + 0.5 * o.norm() * (few_ranks_tolerance(dtype, 5) - ref.HALF_STEP[dtype] + 2.0 ** -23)
     assert (w.detach().cpu().double() - want).norm() <= tol
+
+
+@pytest.mark.gpu
+def test_recorded_many_steps(monkeypatch):
+    """several rounds on narrow matrices in a graph, replayed between eager work"""
+    import dpc_amd
+    bind(monkeypatch, "compiled")
+    prev = dpc_amd._dense_capi.set_library(None)
+    try:
+        gpu = torch.device("cuda")
+        g = [of_rank(s, 3, i).to(gpu) for i, s in enumerate(NARROW)]
+        w, m = [torch.zeros_like(t) for t in g], [torch.zeros_like(t) for t in g]
+        moved, mom = [t.clone() for t in w], [t.clone() for t in m]
+        run = lambda w, m: (dpc_amd.dense.newton_schulz(g, steps=20), dpc_amd.dense.muon_update(w, g, m, lr=0.1, steps=20))[0]
+        want = run([t.clone() for t in w], [t.clone() for t in m])
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            got = run(w, m)
+        for _ in range(3):
+            graph.replay()
+            dpc_amd.dense.newton_schulz(of_rank((60, 64), 0, 3).to(gpu), steps=12)
+            torch.cuda.synchronize()
+            run(moved, mom)
+            assert all(torch.equal(a, b) for a, b in zip(got + w + m, want + moved + mom))
+    finally:
+        dpc_amd._dense_capi.set_library(prev)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("shape,steps", [((1 << 20, 1024), 5), ((64, 1 << 20), 12), ((1 << 20, 3), 5)], ids=["2^20x1024", "64x2^20", "2^20x3"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16], ids=IDS[:2])
+def test_the_longest_sides(monkeypatch, shape, steps, dtype):
+    """2^20, the longest side taken: lines of more than 2^32 bytes, sums of 2^20 terms"""
+    import dpc_amd
+    bind(monkeypatch, "compiled")
+    prev = dpc_amd._dense_capi.set_library(None)
+    try:
+        g = torch.randn(shape, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda").mul_(1e-3).to(dtype)
+        coefficients = DEFAULT if steps == 5 else (2.0, -1.5, 0.5)
+        o = dpc_amd.dense.newton_schulz(g, steps=steps, coefficients=coefficients)
+        want = ref.newton_schulz(g, steps, coefficients)
+        assert ref.off(o, want) <= ref.orthogonal_tolerance(torch.float32, steps) + ref.HALF_STEP[dtype]
+    finally:
+        dpc_amd._dense_capi.set_library(prev)
+        torch.cuda.empty_cache()
