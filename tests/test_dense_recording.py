@@ -82,3 +82,40 @@ def test_recording_beside_a_living_eager_graph_is_refused_by_both_bindings(gpu):
         graph.replay()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("gather", ["none", "accumulate", "copy"])
+def test_a_recorded_training_step_through_either_binding(gpu, gather):
+    """8-bit layers, gradient buckets and Muon in one graph: nothing of an eager step is alive, so nothing is refused"""
+    import dpc_amd
+    from test_dense import toy
+    finals = []
+    for recorded in (False, True):
+        net, x = toy(dpc_amd, gpu), draw((5, 24), 1, torch.float32, gpu)
+        opt = dpc_amd.optim.Muon([net[0].weight, net[2].weight], lr=torch.full((1,), 0.02, device=gpu))
+        red = dpc_amd.distributed.GradBuckets(net.parameters(), bucket_mb=0.001, gather=gather) if gather != "none" else None
+
+        def step():
+            if red is None:
+                opt.zero_grad()
+            loss = net(x).square().sum()
+            loss.backward()
+            if red is not None:
+                red.finish()
+            opt.step()
+            if red is not None:
+                red.zero_()
+            return loss.detach()
+        if recorded:
+            run = dpc_amd.graphs.RecordedStep(step, device=gpu, warmup=3)
+        else:
+            run = step
+            for _ in range(3):
+                step()
+        losses = []
+        for _ in range(3):
+            losses.append(run().clone())
+            torch.cuda.synchronize()
+        finals.append(losses + [p.detach().clone() for p in net.parameters()])
+    assert all(torch.equal(a, b) for a, b in zip(*finals))
